@@ -308,12 +308,54 @@ int tf_lane_attention_paged_static(const void* q, const void* k_new, const void*
                                    int max_window, int max_chunks, int heads, int kv_heads, int head_dim, float scale,
                                    void* stream);
 
+/* The same kind of attention with a sliding window and sinks (no counterpart in the reference): row t of sequence s
+ * stands at slot p = seq_lens[s] + t and sees key j <= p where p - j < window or j < sinks; window 0: every key up to its own
+ * (sinks then change nothing). Keys are cut by absolute position into chunks of chunk_keys (a multiple of 64) that are
+ * attended by themselves and joined in order, so a row's bits depend on chunk_keys and on its own keys only. A call's partials
+ * live in `slots` = tf_window_slots(...) chunks of scratch (tf_window_scratch_bytes). num_pages bounds the page numbers: an entry
+ * outside [0, num_pages) on a page that a row sees is reported as TF_EINVAL through `status` and its keys are left out; entries of
+ * pages that no row sees are not read. max_window bounds a sequence's rows, max_context its keys with its window's own (also
+ * reported). lse, when not NULL, receives ln(sum exp(score)) [rows, heads] fp32. Rows behind seq_start[n_seqs] are left as
+ * they were in out and lse. out, qg, out_packed, group: as below for tf_lane_attention_paged_gated. Keys that no row may see (stale
+ * rows of a page, later rows) may hold anything; a row that sees a value that is not finite has no specified result. */
+int tf_window_slots(int window, int sinks, int max_window, int max_context, int chunk_keys);
+size_t tf_window_scratch_bytes(int rows, int heads, int head_dim, int slots);
+int tf_window_attention(const void* q, const void* k_new, const void* v_new, const void* k_pages, const void* v_pages, int num_pages,
+                        const int* page_table, int max_pages, const int* seq_lens, const int* seq_start, void* out, float* lse,
+                        const void* qg, size_t qg_stride, void* out_packed, int group, void* scratch, size_t scratch_bytes, int rows,
+                        int n_seqs, int max_window, int max_context, int window, int sinks, int chunk_keys, int heads, int kv_heads,
+                        int head_dim, float scale, int* status, void* stream);
+
 /* Commit: copy the first keep[s] window rows of each sequence into its pages at positions
  * seq_lens[s].., for `layers` layers in one launch.
  * Replaces: families/qwen3_5/cuda/forward.py:237-251 (key/value rows in commit). */
 int tf_kv_commit(const void* k_new, const void* v_new, long long rec_stride, void* k_pages, void* v_pages,
                  long long pages_stride, const int* page_table, int max_pages, const int* seq_lens, const int* seq_start,
                  const int* keep, int n_seqs, int layers, int kv_heads, int head_dim, void* stream);
+
+/* ---- a bounded cache: attention weight per key, eviction -------------------------------------------
+ * No counterpart in the reference.
+ * tf_attention_mass: after tf_kv_commit of keep[s] rows, for all `layers` at once: mass[layer, page, kv_head, slot % 16] of every key
+ *   j < seq_lens[s] + keep[s] (seq_lens: before the commit) gains the sum over the kept rows t >= j - seq_lens[s] and the KV head's
+ *   query heads of exp(scale q . k_j - lse), in row order; keys that the commit brought start at that sum and their pos becomes
+ *   row_pos of their row. q [layers, rows, heads, D] bf16 and lse [layers, rows, heads] fp32 are the attention's queries and
+ *   log-sum-exps; k_pages [layers, num_pages, kv_heads, 16, D]; mass fp32 and pos int32 [layers, num_pages, kv_heads, 16].
+ *   A sequence with keep 0 is left as it was.
+ * tf_kv_evict: every sequence of more than `budget` slots is cut back to it, each (layer, KV head) by itself. Kept are the slots
+ *   with pos < sinks or pos >= next_pos[s] - recent, then those of the largest mass (ties to the lower slot, NaN counts as -inf); the i-th kept slot
+ *   at or above the budget moves into the i-th evicted one below it (K, V, mass, pos), the other slots are not touched. moved
+ *   [layers, n_seqs, kv_heads] receives how many moved. seq_lens is not written: the caller's sequences now have
+ *   min(length, budget) slots, whose order no longer follows the text. Pages must belong to one sequence only.
+ *   scratch: tf_evict_scratch_bytes, 4-byte aligned, no initialisation; two launches.
+ * Both report a page number outside [0, num_pages) or a length above max_context as TF_EINVAL through `status` and leave those slots out. */
+int tf_attention_mass(const void* q, const float* lse, const void* k_pages, int num_pages, const int* page_table, int max_pages,
+                      const int* seq_lens, const int* seq_start, const int* keep, const int* row_pos, float* mass, int* pos, int layers,
+                      int rows, int n_seqs, int max_window, int max_context, int heads, int kv_heads, int head_dim, float scale, int* status,
+                      void* stream);
+size_t tf_evict_scratch_bytes(int layers, int n_seqs, int kv_heads, int budget, int max_context);
+int tf_kv_evict(void* k_pages, void* v_pages, int num_pages, const int* page_table, int max_pages, const int* seq_lens, const int* next_pos,
+                float* mass, int* pos, int* moved, void* scratch, size_t scratch_bytes, int layers, int n_seqs, int budget, int recent, int sinks,
+                int max_context, int kv_heads, int head_dim, int* status, void* stream);
 
 /* ---- mixture-of-experts block -------------------------------------------------------------------
  * Replaces: families/qwen4_exp/cuda/moe.py:42-163 (router, select, MoEBuffers, moe) and the combine of
@@ -432,6 +474,23 @@ int tf_topk_sample_rows(const void* x, size_t row_stride, int rows, int vocab, i
  * Replaces: engine/exact_sampling.py:57-109 (uniform_rows, choose_rows), engine/gpu_sampling.py:298-363. */
 int tf_sample_rows(const int* idx, const float* val, int width, const long long* positions, unsigned long long seed,
                    double temperature, int top_k, double top_p, int* tokens, int rows, void* stream);
+
+/* ---- verification of drafted tokens from given random numbers ---------------------------------------
+ * No counterpart in the reference, whose drafts are compared with keyed draws (tf_sample_rows).
+ * Row t of a sequence's window (packed rows seq_start[s] .. seq_start[s + 1] - 1) has the target's logits for the place after it, the
+ * input token of row t + 1 is the draft for that place. With p = softmax(logits row t / temperature) and q = softmax(draft_logits
+ * row t + 1 / draft_temperature), or all of q on the draft itself where draft_logits is NULL, row t + 1 is kept while
+ * uniforms[t][0] * q(draft) < p(draft); keep[s] counts the kept rows with row 0. next[s] is the first token in vocabulary order
+ * whose cumulative weight is above uniforms[t][1] times the total, t the last kept row: the weights are max(p - q, 0) where row t + 1 was
+ * refused (p itself if that leaves nothing), and p where the window was kept whole. A sequence without rows gives keep 0 and next -1, a
+ * row without any probability (every logit -inf or NaN) keeps no draft and gives next -1; +inf counts as the largest bf16
+ * value; a draft outside the vocabulary is refused. uniforms [rows, 2] in [0, 1), fp32 or (uniforms_f64) fp64. logits, draft_logits:
+ * rows of vocab bf16, any alignment, row strides in elements. scratch: tf_verify_scratch_bytes, 8-byte aligned, no initialisation; two launches.
+ * vocab <= 1048576. Acceptances are decided from 32-bit exponentials and 64-bit sums, draws from 64-bit weights and sums. */
+size_t tf_verify_scratch_bytes(int rows, int vocab);
+int tf_verify_rows(const void* logits, size_t row_stride, const void* draft_logits, size_t draft_stride, const int* tokens, const int* seq_start,
+                   const void* uniforms, int uniforms_f64, int* keep, int* next, void* scratch, size_t scratch_bytes, int rows, int vocab,
+                   int n_seqs, double temperature, double draft_temperature, void* stream);
 
 #ifdef __cplusplus
 }

@@ -83,6 +83,19 @@ SIGNATURES: dict[str, tuple] = {
                                                c_float, c_void_p]),
     "tf_kv_commit": (c_int, [c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_void_p,
                              c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p]),
+    "tf_window_slots": (c_int, [c_int, c_int, c_int, c_int, c_int]),
+    "tf_window_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "tf_window_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                    c_void_p, c_void_p, c_size_t, c_void_p, c_int, c_void_p, c_size_t, c_int, c_int, c_int, c_int, c_int,
+                                    c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p]),
+    "tf_attention_mass": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                  c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p]),
+    "tf_evict_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "tf_kv_evict": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+                            c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "tf_verify_scratch_bytes": (c_size_t, [c_int, c_int]),
+    "tf_verify_rows": (c_int, [c_void_p, c_size_t, c_void_p, c_size_t, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                               c_size_t, c_int, c_int, c_int, c_double, c_double, c_void_p]),
     "tf_moe_max_problems": (c_int, [c_int, c_int, c_int]),
     "tf_moe_router": (c_int, [c_void_p, c_size_t, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
     "tf_moe_select": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),

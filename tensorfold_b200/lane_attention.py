@@ -36,6 +36,8 @@ class PagedKV:
         self.table = torch.zeros((n_seqs, max_pages_per_seq), dtype=torch.int32, device=device)
         self.owned = [0] * n_seqs
         self.free = list(range(num_pages - 1, -1, -1))
+        self.holes: set = set()                      # (sequence, page) given back from the middle: release_before
+        self.behind = [0] * n_seqs                   # pages of a sequence that release_before has looked at
 
     def reserve(self, seq: int, tokens: int) -> bool:
         """Make sure sequence ``seq`` owns pages for ``tokens`` positions; True if the table changed."""
@@ -54,8 +56,34 @@ class PagedKV:
 
     def release(self, seq: int) -> None:
         for i in range(self.owned[seq]):
-            self.free.append(int(self.table_host[seq, i]))
+            if (seq, i) not in self.holes:
+                self.free.append(int(self.table_host[seq, i]))
+        self.holes -= {(seq, i) for i in range(self.owned[seq])}
+        self.behind[seq] = 0
         self.owned[seq] = 0
+
+    def release_before(self, seq: int, tokens: int, window: int, sinks: int = 0) -> int:
+        """Give back the pages that no later row of a sequence with ``tokens`` committed positions sees through a sliding window
+        (``lane_window``) and its sinks; how many. Their table entries stay and are not followed any more."""
+
+        first, kept, before = max(0, tokens + 1 - window) // PAGE, -(-sinks // PAGE), len(self.holes)
+        for i in range(max(kept, self.behind[seq]), min(first, self.owned[seq])):
+            self.free.append(int(self.table_host[seq, i]))
+            self.holes.add((seq, i))
+        self.behind[seq] = max(self.behind[seq], first)
+        return len(self.holes) - before
+
+    def shrink(self, seq: int, tokens: int) -> int:
+        """Give back the pages past the first ``tokens`` positions of a sequence (``lane_evict.evict``); how many."""
+
+        before = self.owned[seq]
+        while self.owned[seq] > -(-tokens // PAGE):
+            self.owned[seq] -= 1
+            if (seq, self.owned[seq]) in self.holes:
+                self.holes.discard((seq, self.owned[seq]))
+            else:
+                self.free.append(int(self.table_host[seq, self.owned[seq]]))
+        return before - self.owned[seq]
 
     def sync_table(self) -> None:
         self.table.copy_(self.table_host, non_blocking=True)
