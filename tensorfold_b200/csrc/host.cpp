@@ -302,7 +302,7 @@ PyMethodDef methods[] = {
     TF_FN(tf_moe_combine_peer, 1), TF_FN(tf_moe_pack, 1), TF_FN(tf_moe_act, 1), TF_FN(tf_moe_combine, 1), TF_FN(tf_peer_slot_bytes, 0),
     TF_FN(tf_peer_exchange, 1), TF_FN(tf_qmm_act, 1), TF_FN(tf_swiglu_tiled, 1), TF_FN(tf_qmm_peer, 1), TF_FN(tf_norm_xs_peer, 1),
     TF_FN(tf_set_poll_limit, 0), TF_FN(tf_topk_scratch_bytes, 0), TF_FN(tf_topk_rows, 2), TF_FN(tf_topk_sample_rows, 2), TF_FN(tf_sample_rows, 1),
-    TF_FN(tf_window_slots, 0), TF_FN(tf_window_scratch_bytes, 0), TF_FN(tf_window_attention, 1), TF_FN(tf_attention_mass, 1),
+    TF_FN(tf_window_slots, 0), TF_FN(tf_window_scratch_bytes, 0), TF_FN(tf_window_attention, 2), TF_FN(tf_attention_mass, 1),
     TF_FN(tf_evict_scratch_bytes, 0), TF_FN(tf_kv_evict, 2), TF_FN(tf_verify_scratch_bytes, 0), TF_FN(tf_verify_rows, 2),
     TF_OWN("bound", bound_py), TF_OWN("scratch", scratch_py), TF_OWN("lane_matmul", lane_matmul_py), TF_OWN("prefill_matmul", prefill_matmul_py),
     TF_OWN("current_stream", stream_py), TF_OWN("current_device", device_py), TF_OWN("launch_count", count_py),
