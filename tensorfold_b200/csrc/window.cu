@@ -27,9 +27,22 @@ namespace tf {
 namespace {
 
 constexpr int kPage = 16, kTile = 64, kRows = 128;     // keys a page, keys a tile, query rows a block (the tensor core's M)
-constexpr int kSoftWarps = 4, kMmaWarp = 4, kKWarp = 5, kVWarp = 6, kThreads = 7 * 32;
+constexpr int kSoftWarps = 4, kMmaWarp = 4, kQWarp = 5, kKWarp = 6, kVWarp = 8, kProducers = 2, kThreads = 10 * 32, kSms = 148;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.f;                          // how far (log2) a score may exceed the running maximum
+
+// n / d for 0 <= n < 2^31 without a division: d's reciprocal as a 32-bit fraction, rounded up (exact for n below 2^31 with the
+// shift that makes the fraction's error less than 1 / n).
+struct FastDiv {
+    unsigned d, mul, shift;
+    __device__ int operator()(int n) const { return d == 1 ? n : (int)(__umulhi((unsigned)n, mul) >> shift); }
+};
+inline FastDiv fast_div(int d) {
+    unsigned bits = 0;
+    while ((1ull << bits) < (unsigned long long)d) ++bits;                     // ceil(log2 d)
+    if (d == 1) return {1u, 0u, 0u};
+    return {(unsigned)d, (unsigned)(((1ull << (31 + bits)) + d - 1) / d), bits - 1};
+}
 
 struct WindowArgs {
     const __nv_bfloat16 *q, *k_new, *v_new, *k_pages, *v_pages;
@@ -42,7 +55,9 @@ struct WindowArgs {
     uint8_t* out_packed;               // or null
     int* status;
     int num_pages, max_pages, H, HK, R, S, window, sinks, max_context, max_window, group;
-    int chunk, first_slots, near_slots, qgroups;       // keys a chunk; slots of the sinks' chunks and of the window's
+    int chunk, first_slots, near_slots, slots;         // keys a chunk; slots of the sinks' chunks, of the window's, of both
+    int qgroups, group_rows, items;                    // groups of window rows, rows a group; (group, slot, KV head, sequence) in all
+    FastDiv by_group, by_slot, by_head, by_G, by_chunk;
     float scale_log2;
 };
 
@@ -76,9 +91,9 @@ __device__ __forceinline__ int seq_of(const int* seq_start, int S, int row) {
     return found;
 }
 
-// What a block works on: every thread forms it.
+// One chunk of one (sequence, KV head) for one group of window rows; every role of a block forms it by itself.
 struct Work {
-    int r0, L, p_first, p_last, lo_first, lo_last, nq, key0, head_tiles, far_tile, tiles, sinks;
+    int seq, kvh, slot, t0, r0, n, L, p_first, p_last, lo_first, lo_last, nq, key0, head_tiles, far_tile, tiles, sinks;
     // tile i of the block: those of the sinks, then those of the window
     __device__ int base(int i) const { return key0 + (i < head_tiles ? i : far_tile + i - head_tiles) * kTile; }
     // 0: a committed page that every row sees whole, 1: 16 window rows that every row sees, 2: anything else
@@ -86,30 +101,104 @@ struct Work {
         if (j + kPage > p_first + 1 || !(j >= lo_last || j + kPage <= sinks)) return 2;
         return j + kPage <= L ? 0 : j >= L ? 1 : 2;
     }
-    __device__ bool mixed(int j) const { return kind(j) == 2 || kind(j + kPage) == 2 || kind(j + 2 * kPage) == 2 || kind(j + 3 * kPage) == 2; }
+    // every row sees the tile whole, and no page of it is part committed, part new: nothing to mask, nothing noted
+    __device__ bool plain(int j) const {
+        return j + kTile <= p_first + 1 && (j >= lo_last || j + kTile <= sinks) && !((L & (kPage - 1)) != 0 && j < L && L < j + kTile);
+    }
     __device__ bool any_sees(int j) const { return j <= p_last && (j >= lo_first || j < sinks); }
 };
+struct Raw {           // what a block's next item needs from memory, fetched while the one before it is worked on
+    int r0, r1, L;
+};
+// The row groups of one chunk are neighbours: they read the same keys at the same time.
+__device__ __forceinline__ Raw fetch(const WindowArgs& a, int item) {
+    if (item >= a.items) return {0, 0, 0};
+    const int seq = a.by_head(a.by_slot(a.by_group(item)));
+    return {a.seq_start[seq], a.seq_start[seq + 1], a.seq_lens[seq]};
+}
+__device__ __forceinline__ Work work_of(const WindowArgs& a, int item, Raw raw, bool speaks) {
+    Work w;
+    const int G = (int)a.by_G.d, in_group = a.by_group(item), in_slot = a.by_slot(in_group);
+    w.seq = a.by_head(in_slot);
+    w.kvh = in_slot - w.seq * a.HK;
+    w.slot = in_group - in_slot * a.slots;
+    w.t0 = (item - in_group * a.qgroups) * a.group_rows;
+    w.r0 = raw.r0;
+    w.n = raw.r1 - raw.r0;
+    w.L = raw.L;
+    w.sinks = a.sinks;
+    w.tiles = 0;
+    const int rows = min(a.group_rows, w.n - w.t0);
+    w.nq = rows * G;
+    if (w.n < 1) return w;
+    if (w.n > a.max_window || w.L < 0 || w.L > a.max_context - w.n || w.r0 < 0 || w.r0 > a.R - w.n) {     // not what the call was made for
+        if (speaks) report(a.status, TF_EINVAL);
+        return w;
+    }
+    if (rows < 1) return w;
+    w.p_first = w.L + w.t0;
+    w.p_last = w.p_first + rows - 1;
+    w.lo_first = max(0, w.p_first + 1 - a.window);
+    w.lo_last = max(0, w.p_last + 1 - a.window);
+    int chunk = w.slot;
+    if (chunk >= a.first_slots) {
+        const int lowest = max(a.first_slots, a.by_chunk(max(0, w.L + 1 - a.window)));        // of the sequence: its rows share the slots
+        chunk = lowest + ((w.slot - lowest) % a.near_slots + a.near_slots) % a.near_slots;
+    }
+    w.key0 = chunk * a.chunk;
+    if (w.key0 > w.p_last) return w;
+    const int in_chunk = (min(w.key0 + a.chunk, w.p_last + 1) - w.key0 + kTile - 1) / kTile;
+    w.head_tiles = w.sinks > w.key0 ? min(in_chunk, (w.sinks - w.key0 + kTile - 1) / kTile) : 0;
+    w.far_tile = max(w.head_tiles, w.lo_first > w.key0 ? (w.lo_first - w.key0) / kTile : 0);
+    w.tiles = w.head_tiles + max(0, in_chunk - w.far_tile);
+    return w;
+}
 
 template <int D, int QR>
 struct Cfg {
     static constexpr int SLABS = D / 64;                 // 64 values of a row: one 128-byte swizzle row
     static constexpr int Q_SLAB = QR * 128, Q_BYTES = SLABS * Q_SLAB;
-    static constexpr int TILE_BYTES = kTile * D * 2, K_SLAB = kTile * 128, V_PAGE = kPage * D * 2;
-    static constexpr int FIT = (227 * 1024 - 2048 - Q_BYTES) / TILE_BYTES;
+    static constexpr int TILE_BYTES = kTile * D * 2, K_SLAB = kTile * 128, PAGE_BYTES = kPage * D * 2;
+    static constexpr int STAGE_ROW = 128 + 16, STAGE_BYTES = kSoftWarps * 32 * STAGE_ROW;      // partials on their way out
+    static constexpr int FIT = (227 * 1024 - 2560 - STAGE_BYTES - Q_BYTES) / TILE_BYTES;
     static constexpr int KS = FIT / 2 > 4 ? 4 : FIT / 2, VS = FIT - FIT / 2 > 4 ? 4 : FIT - FIT / 2;
-    static constexpr int NBARS = 2 * KS + 2 * VS + 8 + 1;
-    static constexpr int SMEM = Q_BYTES + (KS + VS) * TILE_BYTES + NBARS * 8 + VS * 8 + 1024;
+    static constexpr int NBARS = 2 * KS + 2 * VS + 8 + 2;
+    static constexpr int SMEM = Q_BYTES + (KS + VS) * TILE_BYTES + STAGE_BYTES + NBARS * 8 + VS * 8 + 1024;
+    // tensor memory: O, two buffers of S, two of P (bf16 pairs)
     static constexpr int O_COL = 0, S_COL = D, P_COL = D + 2 * kTile, COLS = 512;
-    static_assert(KS >= 2 && VS >= 2 && SMEM <= 227 * 1024, "the rings do not fit");
-    static_assert(P_COL + 2 * (kTile / 2) <= COLS, "tensor memory");
+    static_assert(KS >= 2 && SMEM <= 227 * 1024, "the rings do not fit");
+    static_assert(P_COL + kTile <= COLS, "tensor memory");
     // a block of fewer than 128 rows leaves the last rows of the tensor core's Q operand to whatever follows in shared memory
-    static_assert(Q_BYTES - Q_SLAB + kRows * 128 <= Q_BYTES + (KS + VS) * TILE_BYTES, "the operand's rows lie inside the block's memory");
+    static_assert((kRows - QR) * 128 <= (KS + VS) * TILE_BYTES, "the operand's rows lie inside the block's memory");
 };
 
+// two fp32 values in one register pair: one instruction on both
+__device__ __forceinline__ unsigned long long pair_of(float x, float y) {
+    unsigned long long v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    return v;
+}
+__device__ __forceinline__ void split_pair(unsigned long long v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ unsigned long long fma_pair(unsigned long long x, unsigned long long y, unsigned long long z) {
+    unsigned long long v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(x), "l"(y), "l"(z));
+    return v;
+}
+__device__ __forceinline__ unsigned long long add_pair(unsigned long long x, unsigned long long y) {
+    unsigned long long v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
+    return v;
+}
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float v;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(x), "f"(y), "f"(z));
+    return v;
+}
+
 template <int D, int QR>
-__global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_constant__ WindowArgs a, const __grid_constant__ CUtensorMap k_map,
-                                                                   const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap kn_map,
-                                                                   const __grid_constant__ CUtensorMap vn_map) {
+__global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_constant__ WindowArgs a, const __grid_constant__ CUtensorMap q_map,
+                                                                   const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                                                                   const __grid_constant__ CUtensorMap kn_map, const __grid_constant__ CUtensorMap vn_map) {
     using C = Cfg<D, QR>;
     constexpr int KS = C::KS, VS = C::VS, CPR = D / 8;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -118,8 +207,9 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
     uint8_t* q_s = smem + ((1024u - (smem_u32(smem) & 1023u)) & 1023u);
     uint8_t* k_s = q_s + C::Q_BYTES;
     uint8_t* v_s = k_s + KS * C::TILE_BYTES;
-    const uint32_t bars = smem_u32(v_s + VS * C::TILE_BYTES);
-    unsigned long long* bad_s = reinterpret_cast<unsigned long long*>(v_s + VS * C::TILE_BYTES + C::NBARS * 8);
+    uint8_t* stage_s = v_s + VS * C::TILE_BYTES;
+    const uint32_t bars = smem_u32(stage_s + C::STAGE_BYTES);
+    uint32_t* bad_s = reinterpret_cast<uint32_t*>(stage_s + C::STAGE_BYTES + C::NBARS * 8);      // [VS][2]
     auto k_full = [&](int s) { return bars + 8u * s; };
     auto k_empty = [&](int s) { return bars + 8u * (KS + s); };
     auto v_full = [&](int s) { return bars + 8u * (2 * KS + s); };
@@ -128,48 +218,14 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
     auto s_empty = [&](int s) { return bars + 8u * (2 * KS + 2 * VS + 2 + s); };
     auto p_full = [&](int s) { return bars + 8u * (2 * KS + 2 * VS + 4 + s); };
     auto o_done = [&](int s) { return bars + 8u * (2 * KS + 2 * VS + 6 + s); };      // P V of a tile is complete
-    const uint32_t q_full = bars + 8u * (2 * KS + 2 * VS + 8);
-
-    pdl_launch_dependents();
-    pdl_wait();
-    // ---- which chunk, which rows, which tiles ----
-    const int kvh = blockIdx.y, seq = blockIdx.z / a.qgroups, qg = blockIdx.z % a.qgroups, G = a.H / a.HK;
-    Work w;
-    w.r0 = a.seq_start[seq];
-    w.L = a.seq_lens[seq];
-    w.sinks = a.sinks;
-    const int n = a.seq_start[seq + 1] - w.r0;
-    if (n < 1) return;
-    if (n > a.max_window || w.L < 0 || w.L + n > a.max_context || w.r0 < 0 || w.r0 + n > a.R) {     // not what the call was made for
-        if (tid == 0) report(a.status, TF_EINVAL);
-        return;
-    }
-    const int q0 = qg * QR, t_first = q0 / G;
-    if (q0 >= n * G) return;
-    w.nq = min(QR, n * G - q0);
-    w.p_first = w.L + t_first;
-    w.p_last = w.L + (q0 + w.nq - 1) / G;
-    w.lo_first = max(0, w.p_first + 1 - a.window);
-    w.lo_last = max(0, w.p_last + 1 - a.window);
-    const int slot = blockIdx.x;
-    int chunk = slot;
-    if (slot >= a.first_slots) {
-        const int lowest = max(a.first_slots, max(0, w.L + 1 - a.window) / a.chunk);        // of the sequence: its rows share the slots
-        chunk = lowest + ((slot - lowest) % a.near_slots + a.near_slots) % a.near_slots;
-    }
-    w.key0 = chunk * a.chunk;
-    const int end = min(w.key0 + a.chunk, w.p_last + 1), in_chunk = end > w.key0 ? (end - w.key0 + kTile - 1) / kTile : 0;
-    w.head_tiles = w.sinks > w.key0 ? min(in_chunk, (w.sinks - w.key0 + kTile - 1) / kTile) : 0;
-    w.far_tile = max(w.head_tiles, w.lo_first > w.key0 ? (w.lo_first - w.key0) / kTile : 0);
-    w.tiles = w.head_tiles + max(0, in_chunk - w.far_tile);
-    if (w.tiles == 0) return;
-    const int live = (w.nq + 31) / 32;                   // softmax warps with rows
+    const uint32_t q_full = bars + 8u * (2 * KS + 2 * VS + 8), q_empty = q_full + 8;
 
     if (tid == 0) {
-        for (int s = 0; s < KS; ++s) { mbar_init(k_full(s), 1); mbar_init(k_empty(s), 1); }
-        for (int s = 0; s < VS; ++s) { mbar_init(v_full(s), 1); mbar_init(v_empty(s), 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(s_full(s), 1); mbar_init(s_empty(s), live); mbar_init(p_full(s), live); mbar_init(o_done(s), 1); }
-        mbar_init(q_full, kSoftWarps);
+        for (int s = 0; s < KS; ++s) { mbar_init(k_full(s), kProducers); mbar_init(k_empty(s), 1); }
+        for (int s = 0; s < VS; ++s) { mbar_init(v_full(s), kProducers); mbar_init(v_empty(s), 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(s_full(s), 1); mbar_init(s_empty(s), kSoftWarps); mbar_init(p_full(s), kSoftWarps); mbar_init(o_done(s), 1); }
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
         mbar_fence_init();
     }
     if (warp == kMmaWarp) tc_alloc(smem_u32(&tmem_s), C::COLS);
@@ -178,142 +234,213 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
     tc_fence_after();
     const uint32_t tmem = tmem_s;
     Waits wait(a.status);
+    pdl_launch_dependents();
+    pdl_wait();
 
-    if (warp == kKWarp || warp == kVWarp) {
-        // ------------------------------- producers: a warp for K, a warp for V --------------------------------
-        const bool is_v = warp == kVWarp;
+    // All roles go through the block's items and their tiles in the same order and keep step by barriers: nobody is more than a ring ahead.
+    int item = blockIdx.x;
+    Raw raw = fetch(a, item);
+    if (warp >= kKWarp) {
+        // ------------------------------- producers: two warps for K, two for V, half a tile each -----------------------
+        const bool is_v = warp >= kVWarp;
+        const int half = (warp - kKWarp) & 1;
         const CUtensorMap *pages = is_v ? &v_map : &k_map, *rows = is_v ? &vn_map : &kn_map;
         const __nv_bfloat16 *src_pages = is_v ? a.v_pages : a.k_pages, *src_new = is_v ? a.v_new : a.k_new;
-        const int* pt = a.page_table + (size_t)seq * a.max_pages;
+        uint8_t* const ring_s = is_v ? v_s : k_s;
+        const uint32_t full0 = is_v ? v_full(0) : k_full(0), empty0 = is_v ? v_empty(0) : k_empty(0);
+        if (lane == 0) { tma_prefetch_map(pages); tma_prefetch_map(rows); }
         Ring ring(is_v ? VS : KS, 1);
-        for (int i = 0; i < w.tiles; ++i) {
-            const int j0 = w.base(i);
-            const uint32_t full = is_v ? v_full(ring.i) : k_full(ring.i), empty = is_v ? v_empty(ring.i) : k_empty(ring.i);
-            uint8_t* const tile = is_v ? v_s + ring.i * C::TILE_BYTES : k_s + ring.i * C::TILE_BYTES;
-            wait(empty, ring.phase);
-            // the four pages' numbers, looked up together
-            int page = -1;
-            if (lane < 4 && j0 + lane * kPage < w.L && w.any_sees(min(j0 + lane * kPage + kPage - 1, w.p_last)) | w.any_sees(j0 + lane * kPage)) {
-                const int at = (j0 + lane * kPage) / kPage;
-                page = at < a.max_pages ? pt[at] : -1;
-                if (page < 0 || page >= a.num_pages) { report(a.status, TF_EINVAL); page = -1; }
-            }
-            unsigned copied = 0;
+        for (; item < a.items; item += gridDim.x) {
+            const Work w = work_of(a, item, raw, false);
+            raw = fetch(a, item + gridDim.x);
+            const int* pt = a.page_table + (size_t)w.seq * a.max_pages;
+            // page numbers of eight tiles at a time, a lane each, a batch ahead
+            auto numbers = [&](int i) -> int {
+                const int t = i + (lane >> 2);
+                if (t >= w.tiles) return -1;
+                const int j = w.base(t) + (lane & 3) * kPage;
+                if (j >= w.L || !(w.any_sees(min(j + kPage - 1, w.p_last)) || w.any_sees(j))) return -1;      // nobody sees it: not followed
+                const int num = j / kPage < a.max_pages ? pt[j / kPage] : -1;
+                if (num < 0 || num >= a.num_pages) { report(a.status, TF_EINVAL); return -1; }
+                return num;
+            };
+            int now = 0, next = numbers(0);
+            for (int i = 0; i < w.tiles; ++i) {
+                if ((i & 7) == 0) { now = next; next = numbers(i + 8); }
+                const int j0 = w.base(i) + half * 2 * kPage, at = (i & 7) * 4 + half * 2;
+                const int num[2] = {__shfl_sync(0xffffffffu, now, at), __shfl_sync(0xffffffffu, now, at + 1)};
+                const int kinds[2] = {w.kind(j0), w.kind(j0 + kPage)};
+                const bool copy[2] = {kinds[0] == 1 || (kinds[0] == 0 && num[0] >= 0), kinds[1] == 1 || (kinds[1] == 0 && num[1] >= 0)};
+                const uint32_t full = full0 + 8u * ring.i;
+                uint8_t* const tile = ring_s + ring.i * C::TILE_BYTES;
+                wait(empty0 + 8u * ring.i, ring.phase);
+                const bool both = copy[0] && copy[1];
+                if (lane == 0 && (copy[0] || copy[1])) {
+                    if (both) {
+                        if (is_v) bad_s[ring.i * 2 + half] = 0;
+                        mbar_arrive_expect_tx(full, 2 * C::PAGE_BYTES);
+                    } else {
+                        mbar_expect_tx(full, C::PAGE_BYTES);
+                    }
 #pragma unroll
-            for (int pg = 0; pg < 4; ++pg) {
-                const int kind = w.kind(j0 + pg * kPage), num = __shfl_sync(0xffffffffu, page, pg);
-                if (kind == 1 || (kind == 0 && num >= 0)) copied |= 1u << pg;
-            }
-            if (lane == 0 && copied) mbar_expect_tx(full, __popc(copied) * C::V_PAGE);
-            __syncwarp();
-            unsigned long long bad = 0;
-#pragma unroll 1
-            for (int pg = 0; pg < 4; ++pg) {
-                const int j = j0 + pg * kPage, num = __shfl_sync(0xffffffffu, page, pg);
-                if (copied >> pg & 1) {
-                    if (lane == 0) {
-                        const bool committed = w.kind(j) == 0;
-                        const CUtensorMap* map = committed ? pages : rows;
-                        const int y = committed ? (num * a.HK + kvh) * kPage : w.r0 + j - w.L, head = committed ? 0 : kvh;
+                    for (int k = 0; k < 2; ++k) {
+                        if (!copy[k]) continue;
+                        const int pg = half * 2 + k;
+                        const CUtensorMap* map = kinds[k] == 0 ? pages : rows;
+                        const int y = kinds[k] == 0 ? (num[k] * a.HK + w.kvh) * kPage : w.r0 + j0 + k * kPage - w.L, head = kinds[k] == 0 ? 0 : w.kvh;
                         if (is_v) {
-                            tma_4d(smem_u32(tile + pg * C::V_PAGE), map, 0, y, 0, head, full);
+                            tma_4d(smem_u32(tile + pg * C::PAGE_BYTES), map, 0, y, 0, head, full);
                         } else {
 #pragma unroll
                             for (int c = 0; c < C::SLABS; ++c) tma_4d(smem_u32(tile + c * C::K_SLAB + pg * (kPage * 128)), map, 0, y, c, head, full);
                         }
                     }
-                    continue;
                 }
-                // by the warp: lane takes 16-byte column `c` of one or two rows at a time
-                constexpr int RPI = 32 / CPR;
-                const int c = lane % CPR;
-#pragma unroll 4
-                for (int rr = 0; rr < kPage; rr += RPI) {
-                    const int r = rr + lane / CPR, key = j + r;
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (w.any_sees(key)) {
-                        if (key >= w.L) v = *reinterpret_cast<const uint4*>(src_new + ((size_t)(w.r0 + key - w.L) * a.HK + kvh) * D + c * 8);
-                        else if (num >= 0) v = *reinterpret_cast<const uint4*>(src_pages + (((size_t)num * a.HK + kvh) * kPage + r) * D + c * 8);
-                    }
-                    if (is_v) {                          // a value that is not finite: exponent all ones in either half
-                        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-                        bool odd = false;
+                if (!both) {
+                    // by the warp: lane takes 16-byte column `c` of one or two rows at a time; a page's loads before its first store
+                    constexpr int RPI = 32 / CPR, STEPS = kPage / RPI;
+                    const int c = lane % CPR;
+                    uint32_t bad = 0;
+#pragma unroll 1
+                    for (int k = 0; k < 2; ++k) {
+                        if (k == 0 ? copy[0] : copy[1]) continue;
+                        const int number = k == 0 ? num[0] : num[1], key0 = j0 + k * kPage, pg = half * 2 + k;
+                        uint4 v[STEPS];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) odd |= (u[e] & 0x7F80u) == 0x7F80u || (u[e] & 0x7F800000u) == 0x7F800000u;
-                        const unsigned m = __ballot_sync(0xffffffffu, odd);
-                        if (odd) v = make_uint4(0, 0, 0, 0);
+                        for (int x = 0; x < STEPS; ++x) {
+                            const int r = x * RPI + lane / CPR, key = key0 + r;
+                            v[x] = make_uint4(0, 0, 0, 0);
+                            if (!w.any_sees(key)) continue;
+                            if (key >= w.L) v[x] = *reinterpret_cast<const uint4*>(src_new + ((size_t)(w.r0 + key - w.L) * a.HK + w.kvh) * D + c * 8);
+                            else if (number >= 0)
+                                v[x] = *reinterpret_cast<const uint4*>(src_pages + (((size_t)number * a.HK + w.kvh) * kPage + r) * D + c * 8);
+                        }
 #pragma unroll
-                        for (int h = 0; h < RPI; ++h)
-                            if (RPI == 1 ? m != 0 : (m >> (h * CPR) & ((1u << (CPR & 31)) - 1u)) != 0) bad |= 1ull << (pg * kPage + rr + h);
-                        *reinterpret_cast<uint4*>(tile + pg * C::V_PAGE + (c >> 3) * (kPage * 128) + r * 128 + (((c ^ r) & 7) << 4)) = v;
-                    } else {
-                        *reinterpret_cast<uint4*>(tile + (c >> 3) * C::K_SLAB + (pg * kPage + r) * 128 + (((c ^ r) & 7) << 4)) = v;
+                        for (int x = 0; x < STEPS; ++x) {
+                            const int r = x * RPI + lane / CPR;
+                            uint4 u = v[x];
+                            if (is_v) {                  // a value that is not finite: exponent all ones in either half
+                                const uint32_t e[4] = {u.x, u.y, u.z, u.w};
+                                bool odd = false;
+#pragma unroll
+                                for (int y = 0; y < 4; ++y) odd |= (e[y] & 0x7F80u) == 0x7F80u || (e[y] & 0x7F800000u) == 0x7F800000u;
+                                const unsigned m = __ballot_sync(0xffffffffu, odd);
+                                if (odd) u = make_uint4(0, 0, 0, 0);
+                                if (m) {
+#pragma unroll
+                                    for (int h = 0; h < RPI; ++h)
+                                        if (RPI == 1 || (m >> (h * 16) & 0xFFFFu) != 0) bad |= 1u << (k * kPage + x * RPI + h);
+                                }
+                                *reinterpret_cast<uint4*>(tile + pg * C::PAGE_BYTES + (c >> 3) * (kPage * 128) + r * 128 + (((c ^ r) & 7) << 4)) = u;
+                            } else {
+                                *reinterpret_cast<uint4*>(tile + (c >> 3) * C::K_SLAB + (pg * kPage + r) * 128 + (((c ^ r) & 7) << 4)) = u;
+                            }
+                        }
                     }
+                    if (is_v && lane == 0) bad_s[ring.i * 2 + half] = bad;
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(full);
                 }
+                ring.next();
             }
-            if (is_v && lane == 0) bad_s[ring.i] = bad;
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full);
+        }
+    } else if (warp == kQWarp) {
+        // ------------------------------- Q: row = t * G + head, once an item -------------------------------------------
+        Ring ring(1, 1);
+        for (; item < a.items; item += gridDim.x) {
+            const Work w = work_of(a, item, raw, false);
+            raw = fetch(a, item + gridDim.x);
+            if (w.tiles == 0) continue;
+            wait(q_empty, ring.phase);
             ring.next();
+            if (lane == 0) {
+                const int G = (int)a.by_G.d;
+                mbar_arrive_expect_tx(q_full, C::SLABS * a.group_rows * G * 128);
+#pragma unroll
+                for (int c = 0; c < C::SLABS; ++c) tma_4d(smem_u32(q_s + c * C::Q_SLAB), &q_map, 0, w.kvh * G, w.r0 + w.t0, c, q_full);
+            }
+            __syncwarp();
         }
     } else if (warp == kMmaWarp) {
-        // ------------------------------- tensor-core issuer: Q K^T one tile ahead of P V --------------------------
+        // ------------------------------- tensor-core issuer: Q K^T a tile ahead of P V ------------------------------------
         constexpr uint32_t qk_desc = tc_idesc(kTile, false), pv_desc = tc_idesc(D, true);
         const bool leader = elect_one();
         const uint32_t qb = smem_u32(q_s);
-        Ring kr(KS, 0), vr(VS, 0);
-        wait(q_full, 0);
-        for (int i = 0; i <= w.tiles; ++i) {
-            if (i < w.tiles) {
-                const int b = i & 1;
-                wait(s_empty(b), (uint32_t)((i >> 1) & 1) ^ 1u);
-                wait(k_full(kr.i), kr.phase);
-                tc_fence_after();
-                const uint32_t kb = smem_u32(k_s + kr.i * C::TILE_BYTES), d = tmem + C::S_COL + b * kTile;
+        Ring kr(KS, 0), vr(VS, 0), qr(1, 0);
+        int it = 0;                                      // tiles so far, over all items
+        for (; item < a.items; item += gridDim.x) {
+            const Work w = work_of(a, item, raw, false);
+            raw = fetch(a, item + gridDim.x);
+            if (w.tiles == 0) continue;
+            wait(q_full, qr.phase);
+            qr.next();
+            for (int i = 0; i <= w.tiles; ++i) {
+                if (i < w.tiles) {
+                    const int t = it + i, b = t & 1;
+                    wait(s_empty(b), (uint32_t)(((t >> 1) & 1) ^ 1));
+                    wait(k_full(kr.i), kr.phase);
+                    tc_fence_after();
+                    const uint32_t kb = smem_u32(k_s + kr.i * C::TILE_BYTES), d = tmem + C::S_COL + b * kTile;
 #pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks) {
-                    const uint64_t ad = smem_desc(qb + (ks >> 2) * C::Q_SLAB + (ks & 3) * 32), bd = smem_desc(kb + (ks >> 2) * C::K_SLAB + (ks & 3) * 32);
-                    if (leader) tc_mma_ss(d, ad, bd, qk_desc, ks > 0);
+                    for (int ks = 0; ks < D / 16; ++ks) {
+                        const uint64_t ad = smem_desc(qb + (ks >> 2) * C::Q_SLAB + (ks & 3) * 32), bd = smem_desc(kb + (ks >> 2) * C::K_SLAB + (ks & 3) * 32);
+                        if (leader) tc_mma_ss(d, ad, bd, qk_desc, ks > 0);
+                    }
+                    if (leader) {
+                        tc_commit(s_full(b));
+                        tc_commit(k_empty(kr.i));
+                        if (i + 1 == w.tiles) tc_commit(q_empty);
+                    }
+                    kr.next();
+                    __syncwarp();
                 }
-                if (leader) { tc_commit(k_empty(kr.i)); tc_commit(s_full(b)); }
-                kr.next();
-                __syncwarp();
-            }
-            if (i > 0) {
-                const int b = (i - 1) & 1;
-                wait(v_full(vr.i), vr.phase);
-                wait(p_full(b), (uint32_t)(((i - 1) >> 1) & 1));
-                tc_fence_after();
-                const uint32_t vb = smem_u32(v_s + vr.i * C::TILE_BYTES);
+                if (i > 0) {
+                    const int t = it + i - 1, b = t & 1;
+                    wait(v_full(vr.i), vr.phase);
+                    wait(p_full(b), (uint32_t)((t >> 1) & 1));
+                    tc_fence_after();
+                    const uint32_t vb = smem_u32(v_s + vr.i * C::TILE_BYTES);
 #pragma unroll
-                for (int pg = 0; pg < kTile / kPage; ++pg) {
-                    const uint64_t bd = smem_desc_mn(vb + pg * C::V_PAGE, kPage * 128);
-                    if (leader) tc_mma_ts(tmem + C::O_COL, tmem + C::P_COL + b * (kTile / 2) + pg * 8, bd, pv_desc, i > 1 || pg > 0);
+                    for (int pg = 0; pg < kTile / kPage; ++pg) {
+                        const uint64_t bd = smem_desc_mn(vb + pg * C::PAGE_BYTES, kPage * 128);
+                        if (leader) tc_mma_ts(tmem + C::O_COL, tmem + C::P_COL + b * (kTile / 2) + pg * 8, bd, pv_desc, i > 1 || pg > 0);
+                    }
+                    if (leader) { tc_commit(o_done(b)); tc_commit(v_empty(vr.i)); }
+                    vr.next();
+                    __syncwarp();
                 }
-                if (leader) { tc_commit(v_empty(vr.i)); tc_commit(o_done(b)); }
-                vr.next();
-                __syncwarp();
             }
+            it += w.tiles;
         }
     } else {
         // ------------------------------- softmax: thread = query row ---------------------------------------------
-        for (int e = tid; e < w.nq * CPR; e += kSoftWarps * 32) {
-            const int r = e / CPR, c = e % CPR, qr = q0 + r, t = qr / G;
-            const uint4 v = *reinterpret_cast<const uint4*>(a.q + ((size_t)(w.r0 + t) * a.H + kvh * G + qr - t * G) * D + c * 8);
-            *reinterpret_cast<uint4*>(q_s + (c >> 3) * C::Q_SLAB + r * 128 + (((c ^ r) & 7) << 4)) = v;
-        }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_full);
-        if (warp < live) {
-            const int qr = q0 + tid, t = min(qr / G, n - 1), p = w.L + t, lo = max(0, p + 1 - a.window);
-            const uint32_t row = tmem + ((uint32_t)(warp * 32) << 16);
+        const uint32_t row = tmem + ((uint32_t)(warp * 32) << 16);
+        uint8_t* const mine_s = stage_s + warp * 32 * C::STAGE_ROW;
+        const unsigned long long scale2 = pair_of(a.scale_log2, a.scale_log2);
+        Ring vr(VS, 0);
+        int it = 0;
+        for (; item < a.items; item += gridDim.x) {
+            const Work w = work_of(a, item, raw, tid == 0);
+            raw = fetch(a, item + gridDim.x);
+            if (w.tiles == 0) continue;
+            if (warp * 32 >= w.nq) {                     // no rows: keeps step with the others, tile by tile
+                for (int i = 0; i < w.tiles; ++i, ++it, vr.next()) {
+                    wait(s_full(it & 1), (uint32_t)((it >> 1) & 1));
+                    if (it > 1) wait(o_done(it & 1), (uint32_t)((it >> 1) & 1) ^ 1u);
+                    if (lane == 0) { mbar_arrive(s_empty(it & 1)); mbar_arrive(p_full(it & 1)); }
+                }
+                continue;
+            }
+            const bool mine = tid < w.nq;
+            const int G = (int)a.by_G.d, dt = a.by_G(mine ? tid : 0), p = w.p_first + dt, lo = max(0, p + 1 - a.window);
+            const int q_row = (w.r0 + w.t0 + dt) * a.H + w.kvh * G + (mine ? tid : 0) - dt * G;
             float m = -INFINITY, l = 0.f;
-            Ring vr(VS, 0);
-            for (int i = 0; i < w.tiles; ++i) {
-                const int b = i & 1, j0 = w.base(i);
-                const uint32_t round = (uint32_t)((i >> 1) & 1);
+#pragma unroll 1
+            for (int i = 0; i < w.tiles; ++i, ++it) {
+                const int b = it & 1, j0 = w.base(i);
+                const uint32_t round = (uint32_t)((it >> 1) & 1);
+                const bool plain = w.plain(j0);
                 wait(s_full(b), round);
                 tc_fence_after();
                 float s[kTile];
@@ -323,28 +450,28 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_empty(b));
-                unsigned long long bad = 0;
-                if (w.mixed(j0)) {                       // the V tile's notes are there once it is (and stay until P V)
+                if (!plain) {                            // the V tile's notes are there once it is (and stay until P V)
                     wait(v_full(vr.i), vr.phase);
-                    bad = bad_s[vr.i];
+                    const uint32_t bad[2] = {bad_s[vr.i * 2], bad_s[vr.i * 2 + 1]};
+                    // bit e: the row sees key j0 + e; up to p, and from lo on or below the sinks' end
+                    auto below = [](int x) -> unsigned long long { return x <= 0 ? 0ull : x >= kTile ? ~0ull : (1ull << x) - 1; };
+                    const unsigned long long sees = below(p + 1 - j0) & (~below(lo - j0) | below(w.sinks - j0));
+                    const uint32_t see[2] = {(uint32_t)sees, (uint32_t)(sees >> 32)};
+                    if ((see[0] & bad[0]) | (see[1] & bad[1])) l = __int_as_float(0x7FC00000);
+#pragma unroll
+                    for (int e = 0; e < kTile; ++e) s[e] = see[e >> 5] >> (e & 31) & 1 ? s[e] : -INFINITY;
                 }
                 vr.next();
-                const bool whole = j0 + kTile <= p + 1 && (j0 >= lo || j0 + kTile <= w.sinks);
-                float top = -INFINITY;
-                if (__all_sync(0xffffffffu, whole) && bad == 0) {
+                float tops[4];
 #pragma unroll
-                    for (int e = 0; e < kTile; ++e) top = fmaxf(top, s[e]);
-                } else {
+                for (int e = 0; e < 4; ++e) tops[e] = s[e];
 #pragma unroll
-                    for (int e = 0; e < kTile; ++e) {
-                        const int j = j0 + e;
-                        const bool sees = j <= p && (j >= lo || j < w.sinks);
-                        s[e] = sees ? s[e] : -INFINITY;
-                        if (sees && (bad >> e & 1)) l = __int_as_float(0x7FC00000);
-                        top = fmaxf(top, s[e]);
-                    }
+                for (int e = 4; e + 7 < kTile + 4; e += 8) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (e + 2 * k + 1 < kTile) tops[k] = max3(tops[k], s[e + 2 * k], s[e + 2 * k + 1]);
                 }
-                top *= a.scale_log2;
+                const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * a.scale_log2;
                 // move the maximum only where it must: a row's choice looks at its own scores alone
                 float alpha = 1.f;
                 if (top > m + kSlack || (m == -INFINITY && top > m)) {
@@ -352,9 +479,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
                     m = top;
                     l *= alpha;
                 }
-                const float off = m == -INFINITY ? 0.f : m;
                 if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-                    wait(o_done((i - 1) & 1), (uint32_t)(((i - 1) >> 1) & 1));
+                    wait(o_done((it - 1) & 1), (uint32_t)(((it - 1) >> 1) & 1));
                     tc_fence_after();
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
@@ -366,19 +492,25 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
                         for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(o[e] * alpha);
                         tc_st32(row + C::O_COL + c, u);
                     }
-                    tc_wait_st();
                 }
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                const float off = m == -INFINITY ? 0.f : -m;
+                const unsigned long long off2 = pair_of(off, off);
+                unsigned long long sum[4] = {0, 0, 0, 0};            // two zeros each
                 uint32_t pk[kTile / 2];
 #pragma unroll
                 for (int e = 0; e < kTile; e += 2) {
-                    const float x = fast_exp2(fmaf(s[e], a.scale_log2, -off)), y = fast_exp2(fmaf(s[e + 1], a.scale_log2, -off));
-                    sum[(e >> 1) & 3] += x;
-                    sum[(e >> 1) & 3] += y;
-                    pk[e >> 1] = pack_bf16(x, y);
+                    float x, y;
+                    split_pair(fma_pair(pair_of(s[e], s[e + 1]), scale2, off2), x, y);
+                    x = fast_exp2(x);
+                    y = fast_exp2(y);
+                    sum[(e >> 1) & 3] = add_pair(sum[(e >> 1) & 3], pair_of(x, y));
+                    const __nv_bfloat162 xy = __floats2bfloat162_rn(x, y);
+                    pk[e >> 1] = *reinterpret_cast<const uint32_t*>(&xy);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                if (i > 1) wait(o_done(b), round ^ 1u);       // P V of tile i - 2 has read this buffer
+                float s0, s1;
+                split_pair(add_pair(add_pair(sum[0], sum[1]), add_pair(sum[2], sum[3])), s0, s1);
+                l += s0 + s1;
+                if (it > 1) wait(o_done(b), round ^ 1u);             // P V of the tile before last has read this buffer
                 tc_fence_after();
                 tc_st32(row + C::P_COL + b * (kTile / 2), pk);
                 tc_wait_st();
@@ -387,21 +519,37 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
                 if (lane == 0) mbar_arrive(p_full(b));
             }
             // ---- the chunk's partials ----
-            wait(o_done((w.tiles - 1) & 1), (uint32_t)(((w.tiles - 1) >> 1) & 1));
-            tc_fence_after();
-            const size_t cell = ((size_t)slot * a.R + w.r0 + t) * a.H + kvh * G + qr - t * G;
-            const bool mine = tid < w.nq;
-            if (mine) { a.part_m[cell] = m; a.part_l[cell] = l; }
-#pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-                float o[32];
-                tc_ld32(row + C::O_COL + c, o);
-                tc_wait_ld();
-                if (mine) {
+            const size_t first = (size_t)w.slot * a.R * a.H;
+            if (mine) { a.part_m[first + q_row] = m; a.part_l[first + q_row] = l; }
+            // 32 values of 32 rows at a time through shared memory, so that a store covers whole lines; a lane's rows are 4 x + lane / 8
+            const int rows_here = min(32, w.nq - warp * 32);
+            float* to[8];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(a.part_o + cell * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            for (int x = 0; x < 8; ++x) to[x] = a.part_o + (first + __shfl_sync(0xffffffffu, q_row, x * 4 + (lane >> 3))) * D + (lane & 7) * 4;
+            wait(o_done((it - 1) & 1), (uint32_t)(((it - 1) >> 1) & 1));
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D; c += 64) {
+                float o[2][32];
+                tc_ld32(row + C::O_COL + c, o[0]);
+                tc_ld32(row + C::O_COL + c + 32, o[1]);
+                tc_wait_ld();
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<float4*>(mine_s + lane * C::STAGE_ROW + e * 4) = make_float4(o[h][e], o[h][e + 1], o[h][e + 2], o[h][e + 3]);
+                    __syncwarp();
+                    float4 v[8];
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) v[x] = *reinterpret_cast<const float4*>(mine_s + (x * 4 + (lane >> 3)) * C::STAGE_ROW + (lane & 7) * 16);
+#pragma unroll
+                    for (int x = 0; x < 8; ++x)
+                        if (x * 4 + (lane >> 3) < rows_here) *reinterpret_cast<float4*>(to[x] + c + h * 32) = v[x];
+                    __syncwarp();
                 }
             }
+            tc_fence_before();                           // the sums have been read: the next item's may overwrite them
         }
     }
     tc_fence_before();
@@ -436,8 +584,8 @@ __global__ void __launch_bounds__(128) window_join_kernel(const WindowArgs a) {
     if (p < 0 || p >= a.max_context) return;                           // reported by the chunk kernel
     const int lo = max(0, p + 1 - a.window);
     // chunks with sinks below the window, then the window's
-    const int head_chunks = min(a.sinks, lo) > 0 ? (min(a.sinks, lo) - 1) / a.chunk + 1 : 0;
-    const int far = max(head_chunks, lo / a.chunk), count = head_chunks + p / a.chunk + 1 - far;
+    const int head_chunks = min(a.sinks, lo) > 0 ? a.by_chunk(min(a.sinks, lo) - 1) + 1 : 0;
+    const int far = max(head_chunks, a.by_chunk(lo)), count = head_chunks + a.by_chunk(p) + 1 - far;
     float acc[8], m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = 0.f;
@@ -488,9 +636,10 @@ __global__ void __launch_bounds__(128) window_join_kernel(const WindowArgs a) {
 }
 
 // ---- host side -----------------------------------------------------------------------------------------
-// Descriptors of the tiled copies: rows of D values seen as [row][64 values][D / 64 slabs], a box of 16 rows and one slab (K, whose
-// slabs lie apart in a tile) or all of them (V).
-bool describe(CUtensorMap* map, const void* base, unsigned long long rows, size_t row_bytes, int heads, size_t head_bytes, int D, bool all_slabs) {
+// Descriptor of a tiled copy of rows of D values: (64 values, rows, outer, D / 64 slabs), or with the slabs before `outer`; a box is
+// box_rows rows of box_outer outer places and of one slab (K and Q, whose slabs lie apart in shared memory) or all of them (V).
+bool describe(CUtensorMap* map, const void* base, int D, unsigned long long rows, size_t row_bytes, unsigned long long outer, size_t outer_bytes,
+              bool slabs_last, int box_rows, int box_outer, int box_slabs) {
     static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
         void* fn = nullptr;
         cudaDriverEntryPointQueryResult got;
@@ -499,15 +648,17 @@ bool describe(CUtensorMap* map, const void* base, unsigned long long rows, size_
         return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
     }();
     if (encode == nullptr) return false;
-    const cuuint64_t dims[4] = {64, rows < 16 ? 16 : rows, (cuuint64_t)(D / 64), (cuuint64_t)heads};
-    const cuuint64_t strides[3] = {row_bytes, 128, head_bytes};
-    const cuuint32_t box[4] = {64, kPage, all_slabs ? (cuuint32_t)(D / 64) : 1u, 1}, steps[4] = {1, 1, 1, 1};
+    const int o = slabs_last ? 2 : 3, c = slabs_last ? 3 : 2;
+    cuuint64_t dims[4] = {64, rows, 0, 0}, strides[3] = {row_bytes, 0, 0};
+    cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 0, 0}, steps[4] = {1, 1, 1, 1};
+    dims[o] = outer; strides[o - 1] = outer_bytes; box[o] = (cuuint32_t)box_outer;
+    dims[c] = (cuuint64_t)(D / 64); strides[c - 1] = 128; box[c] = (cuuint32_t)box_slabs;
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int D, int QR>
-int launch_chunks(WindowArgs& a, int slots, cudaStream_t st) {
+int launch_chunks(const WindowArgs& a, cudaStream_t st) {
     using C = Cfg<D, QR>;
     static bool configured[64] = {};       // the opt-in is per device
     int dev = 0;
@@ -519,16 +670,17 @@ int launch_chunks(WindowArgs& a, int slots, cudaStream_t st) {
         }
         configured[dev] = true;
     }
-    CUtensorMap maps[4];
-    const unsigned long long rows = (unsigned long long)a.num_pages * a.HK * kPage;
+    CUtensorMap maps[5];
+    const int G = a.H / a.HK;
+    const unsigned long long H = a.H, HK = a.HK, R = a.R, rows = (unsigned long long)a.num_pages * HK * kPage;
     const size_t row = (size_t)D * 2;
-    if (!describe(&maps[0], a.k_pages, rows, row, 1, row, D, false) || !describe(&maps[1], a.v_pages, rows, row, 1, row, D, true) ||
-        !describe(&maps[2], a.k_new, a.R, row * a.HK, a.HK, row, D, false) || !describe(&maps[3], a.v_new, a.R, row * a.HK, a.HK, row, D, true))
+    if (!describe(&maps[0], a.q, D, H, row, R, row * H, true, G, a.group_rows, 1) ||
+        !describe(&maps[1], a.k_pages, D, rows, row, 1, row, false, kPage, 1, 1) || !describe(&maps[2], a.v_pages, D, rows, row, 1, row, false, kPage, 1, D / 64) ||
+        !describe(&maps[3], a.k_new, D, R < 16 ? 16 : R, row * HK, HK, row, false, kPage, 1, 1) ||
+        !describe(&maps[4], a.v_new, D, R < 16 ? 16 : R, row * HK, HK, row, false, kPage, 1, D / 64))
         return TF_ECUDA;
-    a.qgroups = (int)(((long long)a.max_window * (a.H / a.HK) + QR - 1) / QR);
-    if ((long long)a.S * a.qgroups > 65535) return TF_EINVAL;
-    void* args[] = {&a, &maps[0], &maps[1], &maps[2], &maps[3]};
-    if (launch_pdl((const void*)window_chunk_kernel<D, QR>, dim3(slots, a.HK, a.S * a.qgroups), dim3(kThreads), C::SMEM, st, args) != cudaSuccess) {
+    void* args[] = {const_cast<WindowArgs*>(&a), &maps[0], &maps[1], &maps[2], &maps[3], &maps[4]};
+    if (launch_pdl((const void*)window_chunk_kernel<D, QR>, dim3(a.items < kSms ? a.items : kSms), dim3(kThreads), C::SMEM, st, args) != cudaSuccess) {
         cudaGetLastError();
         return TF_ECUDA;
     }
@@ -536,13 +688,20 @@ int launch_chunks(WindowArgs& a, int slots, cudaStream_t st) {
 }
 
 template <int D>
-int run(WindowArgs& a, int slots, cudaStream_t st) {
-    const bool small = a.max_window * (long long)(a.H / a.HK) <= 64;
-    const int rc = small ? launch_chunks<D, 64>(a, slots, st) : launch_chunks<D, 128>(a, slots, st);
+int run(WindowArgs& a, cudaStream_t st) {
+    const int G = a.H / a.HK, most = kRows / G;
+    a.group_rows = a.max_window < most ? a.max_window : most;
+    if (a.group_rows > a.R) a.group_rows = a.R;
+    a.qgroups = (a.max_window + a.group_rows - 1) / a.group_rows;
+    const long long items = (long long)a.qgroups * a.slots * a.HK * a.S;
+    if (items > (1 << 30)) return TF_EINVAL;
+    a.items = (int)items;
+    a.by_group = fast_div(a.qgroups); a.by_slot = fast_div(a.slots); a.by_head = fast_div(a.HK); a.by_G = fast_div(G); a.by_chunk = fast_div(a.chunk);
+    const int rc = a.group_rows * G <= 64 ? launch_chunks<D, 64>(a, st) : launch_chunks<D, 128>(a, st);
     if (rc != TF_OK) return rc;
-    void* args[] = {&a};
-    const int heads = 4 * (32 / (D / 8)), rows = a.out_packed ? tf_padded_rows(a.R) : a.R;
-    if (launch_pdl((const void*)window_join_kernel<D>, dim3((a.H + heads - 1) / heads, rows), dim3(128), 0, st, args) != cudaSuccess) {
+    void* join[] = {&a};
+    const int heads = 4 * (32 / (D / 8)), out_rows = a.out_packed ? tf_padded_rows(a.R) : a.R;
+    if (launch_pdl((const void*)window_join_kernel<D>, dim3((a.H + heads - 1) / heads, out_rows), dim3(128), 0, st, join) != cudaSuccess) {
         cudaGetLastError();
         return TF_ECUDA;
     }
@@ -594,7 +753,7 @@ int tf_window_attention(const void* q, const void* k_new, const void* v_new, con
     a.window = window > 0 ? window : 1 << 30; a.sinks = window > 0 ? sinks : 0; a.max_context = max_context; a.group = group;
     a.scale_log2 = scale * tf::kLog2e;
     a.max_window = max_window;
-    a.chunk = chunk_keys;
+    a.chunk = chunk_keys; a.slots = slots;
     const tf::Slots cut = tf::slots_for(window, sinks, max_window, max_context, chunk_keys);
     a.first_slots = cut.first; a.near_slots = cut.near > 0 ? cut.near : 1;
     const size_t cells = (size_t)slots * rows * heads;
@@ -602,7 +761,7 @@ int tf_window_attention(const void* q, const void* k_new, const void* v_new, con
     a.part_m = a.part_o + cells * head_dim;
     a.part_l = a.part_m + cells;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return head_dim == 256 ? tf::run<256>(a, slots, st) : tf::run<128>(a, slots, st);
+    return head_dim == 256 ? tf::run<256>(a, st) : tf::run<128>(a, st);
 }
 
 }  // extern "C"
