@@ -17,6 +17,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <atomic>
+#include <cmath>
 #include <cstring>
 #include <map>
 #include <mutex>
@@ -276,6 +277,209 @@ PyObject* prefill_matmul_py(PyObject* const* args, Py_ssize_t) {
     return shaped(out, x, n);
 }
 
+// ---- the calls of a bounded cache and of draft verification: checks, allocations and launches in one native call -----------------
+// Their device work is 5 to 20 us on small calls; the same steps from Python took 15 to 20.
+
+// Arguments that must hold, with the text of the ValueError where one does not.
+void need(bool ok, const char* text) {
+    if (!ok) fail(PyExc_ValueError, text);
+}
+at::Tensor optional_tensor(PyObject* o) { return o == Py_None ? at::Tensor() : tensor(o); }
+bool plain(const at::Tensor& t, at::ScalarType type) { return t.scalar_type() == type && t.is_contiguous(); }
+template <class... T>
+void on_device(const at::Tensor& first, const T&... others) {
+    const auto is_cuda = [](const at::Tensor& t) { return !t.defined() || t.is_cuda(); };
+    need(first.is_cuda() && (is_cuda(others) && ...), "lane kernels take CUDA tensors only (there is no CPU path)");
+    need(((!others.defined() || others.device() == first.device()) && ...), "the tensors must be on one device");
+}
+template <class T>
+T* data_of(const at::Tensor& t) { return t.defined() ? static_cast<T*>(t.mutable_data_ptr()) : nullptr; }
+// The caller's buffer or one of `bytes` from the allocator. (A buffer that is too small is refused by the entry point.)
+at::Tensor buffer(PyObject* given, size_t bytes, const at::Tensor& like) {
+    if (given != Py_None) return tensor(given);
+    return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+}
+size_t bytes_of(const at::Tensor& t) { return (size_t)t.numel() * t.element_size(); }
+int32_t checked_int(PyObject* o, const char* text) {
+    const long long v = convert<long long>(o);
+    need(v >= INT32_MIN && v <= INT32_MAX, text);
+    return (int32_t)v;
+}
+
+// window_attention(q, k_new, v_new, k_pages, v_pages, page_table, seq_lens, seq_start, scale, max_window, max_context, window (0: none), sinks,
+//                  chunk_keys, scratch, out, lse, gate, packed data, packed group, status) -> out or None
+PyObject* window_attention_py(PyObject* const* args, Py_ssize_t n) {
+    if (n != 21) fail(PyExc_TypeError, "window_attention takes 21 arguments");
+    at::AutoDispatchBelowADInplaceOrView no_grad;
+    const at::Tensor q = tensor(args[0]), k_new = tensor(args[1]), v_new = tensor(args[2]), k_pages = tensor(args[3]), v_pages = tensor(args[4]),
+                     table = tensor(args[5]), lens = tensor(args[6]), start = tensor(args[7]), lse = optional_tensor(args[16]),
+                     gate = optional_tensor(args[17]), packed = optional_tensor(args[18]);
+    at::Tensor out = optional_tensor(args[15]);
+    const double scale = convert<double>(args[8]);
+    const char* sizes = "window >= 1 (or None), sinks >= 0, chunk_keys a positive multiple of 64 and max_context >= max_window >= 1 required";
+    const int max_window = checked_int(args[9], sizes), max_context = checked_int(args[10], sizes), window = checked_int(args[11], sizes),
+              sinks = checked_int(args[12], sizes), chunk = checked_int(args[13], sizes), group = convert<int>(args[19]);
+    on_device(q, k_new, v_new, k_pages, v_pages, table, lens, start, lse, gate, packed, out, args[14] == Py_None ? at::Tensor() : tensor(args[14]));
+    need(q.dim() == 3 && k_new.dim() == 3 && k_pages.dim() == 4 && table.dim() == 2 && lens.dim() == 1 && start.dim() == 1, "unsupported attention shape");
+    const int64_t r = q.size(0), h = q.size(1), d = q.size(2), hk = k_new.size(1), s = lens.size(0);
+    need(r >= 1 && s >= 1 && h >= 1 && hk >= 1 && k_new.size(0) == r && k_new.size(2) == d && v_new.sizes() == k_new.sizes() && (d == 128 || d == 256) && h % hk == 0 &&
+             h / hk <= 16 && k_pages.size(0) >= 1 && k_pages.size(1) == hk && k_pages.size(2) == 16 && k_pages.size(3) == d && v_pages.sizes() == k_pages.sizes() &&
+             table.size(0) == s && table.size(1) >= 1 && start.size(0) == s + 1 && r <= 65535 && s <= 65535 && h <= 65535 && k_pages.size(0) <= INT32_MAX &&
+             table.size(1) <= INT32_MAX,
+         "unsupported attention shape");
+    need(plain(q, at::kBFloat16) && plain(k_new, at::kBFloat16) && plain(v_new, at::kBFloat16) && plain(k_pages, at::kBFloat16) && plain(v_pages, at::kBFloat16),
+         "attention tensors must be contiguous bf16");
+    need(plain(table, at::kInt) && plain(lens, at::kInt) && plain(start, at::kInt), "page_table, seq_lens and seq_start must be contiguous int32");
+    need(scale > 0 && scale < INFINITY, "scale must be positive and finite");
+    const int slots = tf_window_slots(window, sinks, max_window, max_context, chunk);
+    need(slots > 0, sizes);
+    need(!lse.defined() || (plain(lse, at::kFloat) && lse.dim() == 2 && lse.size(0) == r && lse.size(1) == h), "lse must be contiguous float32 (R, H)");
+    need(!out.defined() || (plain(out, at::kBFloat16) && out.sizes() == q.sizes()), "out must be contiguous bf16 (R, H, D)");
+    need(!gate.defined() || (gate.scalar_type() == at::kBFloat16 && gate.dim() == 2 && gate.size(0) == r && gate.size(1) == h * 2 * d && gate.stride(1) == 1),
+         "gate must be the (R, H * 2 * D) bf16 rows of the q projection");
+    const c10::cuda::CUDAGuard on(q.device());
+    const auto stream = c10::cuda::getCurrentCUDAStream(q.device().index());
+    const at::Tensor scratch = buffer(args[14], tf_window_scratch_bytes((int)r, (int)h, (int)d, slots), q);
+    if (!out.defined() && !packed.defined()) out = at::empty_like(q);
+    int* status = convert<int*>(args[20]);
+    const int rc = [&] {
+        const Released unlocked;
+        return tf_window_attention(q.const_data_ptr(), k_new.const_data_ptr(), v_new.const_data_ptr(), k_pages.const_data_ptr(), v_pages.const_data_ptr(),
+                                   (int)k_pages.size(0), data_of<int>(table), (int)table.size(1), data_of<int>(lens), data_of<int>(start), data_of<void>(out),
+                                   data_of<float>(lse), data_of<void>(gate), gate.defined() ? (size_t)gate.stride(0) : 0, data_of<void>(packed), group,
+                                   scratch.mutable_data_ptr(), bytes_of(scratch), (int)r, (int)s, max_window, max_context, window, sinks, chunk, (int)h, (int)hk,
+                                   (int)d, (float)scale, status, stream.stream());
+    }();
+    check_rc(rc, "window_attention");
+    g_launches.fetch_add(2, std::memory_order_relaxed);
+    if (!out.defined()) Py_RETURN_NONE;
+    return THPVariable_Wrap(out);
+}
+
+// pages [layers, pages, HK, 16, D] with the planes mass and pos, and the sequences' table and lengths
+void check_cache(const at::Tensor& k_pages, const at::Tensor& mass, const at::Tensor& pos, const at::Tensor& table, const at::Tensor& lens) {
+    need(k_pages.dim() == 5 && k_pages.size(0) >= 1 && k_pages.size(1) >= 1 && k_pages.size(2) >= 1 && k_pages.size(3) == 16 &&
+             (k_pages.size(4) == 128 || k_pages.size(4) == 256) && plain(k_pages, at::kBFloat16) && k_pages.size(0) <= 65535 && k_pages.size(1) <= INT32_MAX &&
+             k_pages.size(2) <= 65535,
+         "the pages must be contiguous bf16 (layers, pages, HK, 16, D), D 128 or 256");
+    const auto cells = k_pages.sizes().slice(0, 4);
+    need(mass.sizes() == cells && pos.sizes() == cells && plain(mass, at::kFloat) && plain(pos, at::kInt),
+         "mass must be contiguous float32 and pos int32, (layers, pages, HK, 16)");
+    need(table.dim() == 2 && lens.dim() == 1 && table.size(0) == lens.size(0) && lens.size(0) >= 1 && lens.size(0) <= 65535 && table.size(1) >= 1 &&
+             table.size(1) <= INT32_MAX,
+         "page_table must be (S, max_pages) and seq_lens (S,)");
+    need(plain(table, at::kInt) && plain(lens, at::kInt), "page_table, lengths, positions and counts must be contiguous int32");
+}
+
+// attention_mass(q, lse, k_pages, page_table, seq_lens, seq_start, keep, row_pos, mass, pos, scale, max_window, max_context, status)
+PyObject* attention_mass_py(PyObject* const* args, Py_ssize_t n) {
+    if (n != 14) fail(PyExc_TypeError, "attention_mass takes 14 arguments");
+    at::AutoDispatchBelowADInplaceOrView no_grad;
+    const at::Tensor q = tensor(args[0]), lse = tensor(args[1]), k_pages = tensor(args[2]), table = tensor(args[3]), lens = tensor(args[4]), start = tensor(args[5]),
+                     keep = tensor(args[6]), row_pos = tensor(args[7]), mass = tensor(args[8]), pos = tensor(args[9]);
+    const double scale = convert<double>(args[10]);
+    const char* sizes = "scale must be positive and finite, max_context >= max_window >= 1";
+    const int max_window = checked_int(args[11], sizes), max_context = checked_int(args[12], sizes);
+    on_device(q, lse, k_pages, table, lens, start, keep, row_pos, mass, pos);
+    check_cache(k_pages, mass, pos, table, lens);
+    const int64_t layers = k_pages.size(0), hk = k_pages.size(2), d = k_pages.size(4), s = lens.size(0);
+    need(q.dim() == 4 && q.size(0) == layers && q.size(1) >= 1 && q.size(1) <= INT32_MAX && q.size(3) == d && plain(q, at::kBFloat16),
+         "q must be contiguous bf16 (layers, R, H, D)");
+    const int64_t r = q.size(1), h = q.size(2);
+    need(h >= 1 && h % hk == 0 && h / hk <= 16, "H must be a multiple of HK, at most 16 heads a KV head");
+    need(lse.dim() == 3 && lse.size(0) == layers && lse.size(1) == r && lse.size(2) == h && plain(lse, at::kFloat), "lse must be contiguous float32 (layers, R, H)");
+    need(start.dim() == 1 && start.size(0) == s + 1 && keep.dim() == 1 && keep.size(0) == s && row_pos.dim() == 1 && row_pos.size(0) == r && plain(start, at::kInt) &&
+             plain(keep, at::kInt) && plain(row_pos, at::kInt),
+         "seq_start (S+1,), keep (S,) and row_pos (R,), contiguous int32, required");
+    need(scale > 0 && scale < INFINITY && max_window >= 1 && max_context >= max_window, sizes);
+    const c10::cuda::CUDAGuard on(q.device());
+    const auto stream = c10::cuda::getCurrentCUDAStream(q.device().index());
+    int* status = convert<int*>(args[13]);
+    const int rc = [&] {
+        const Released unlocked;
+        return tf_attention_mass(q.const_data_ptr(), data_of<float>(lse), k_pages.const_data_ptr(), (int)k_pages.size(1), data_of<int>(table), (int)table.size(1),
+                                 data_of<int>(lens), data_of<int>(start), data_of<int>(keep), data_of<int>(row_pos), data_of<float>(mass), data_of<int>(pos),
+                                 (int)layers, (int)r, (int)s, max_window, max_context, (int)h, (int)hk, (int)d, (float)scale, status, stream.stream());
+    }();
+    check_rc(rc, "attention_mass");
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    Py_RETURN_NONE;
+}
+
+// evict(k_pages, v_pages, page_table, seq_lens, next_pos, mass, pos, budget, recent, sinks, max_context, scratch, status) -> moved
+PyObject* evict_py(PyObject* const* args, Py_ssize_t n) {
+    if (n != 13) fail(PyExc_TypeError, "evict takes 13 arguments");
+    at::AutoDispatchBelowADInplaceOrView no_grad;
+    const at::Tensor k_pages = tensor(args[0]), v_pages = tensor(args[1]), table = tensor(args[2]), lens = tensor(args[3]), next_pos = tensor(args[4]),
+                     mass = tensor(args[5]), pos = tensor(args[6]);
+    const char* sizes = "budget >= recent + sinks, all non-negative, budget and max_context at least 1";
+    const int budget = checked_int(args[7], sizes), recent = checked_int(args[8], sizes), sinks = checked_int(args[9], sizes), max_context = checked_int(args[10], sizes);
+    on_device(k_pages, v_pages, table, lens, next_pos, mass, pos, args[11] == Py_None ? at::Tensor() : tensor(args[11]));
+    check_cache(k_pages, mass, pos, table, lens);
+    const int64_t layers = k_pages.size(0), hk = k_pages.size(2), d = k_pages.size(4), s = lens.size(0);
+    need(v_pages.sizes() == k_pages.sizes() && plain(v_pages, at::kBFloat16) && next_pos.dim() == 1 && next_pos.size(0) == s && plain(next_pos, at::kInt),
+         "v_pages must match k_pages and next_pos be (S,) int32");
+    need(budget >= 1 && recent >= 0 && sinks >= 0 && (int64_t)recent + sinks <= budget && max_context >= 1, sizes);
+    const c10::cuda::CUDAGuard on(k_pages.device());
+    const auto stream = c10::cuda::getCurrentCUDAStream(k_pages.device().index());
+    const at::Tensor scratch = buffer(args[11], tf_evict_scratch_bytes((int)layers, (int)s, (int)hk, budget, max_context), k_pages);
+    const at::Tensor moved = at::empty({layers, s, hk}, k_pages.options().dtype(at::kInt));
+    int* status = convert<int*>(args[12]);
+    const int rc = [&] {
+        const Released unlocked;
+        return tf_kv_evict(data_of<void>(k_pages), data_of<void>(v_pages), (int)k_pages.size(1), data_of<int>(table), (int)table.size(1), data_of<int>(lens),
+                           data_of<int>(next_pos), data_of<float>(mass), data_of<int>(pos), data_of<int>(moved), scratch.mutable_data_ptr(), bytes_of(scratch), (int)layers,
+                           (int)s, budget, recent, sinks, max_context, (int)hk, (int)d, status, stream.stream());
+    }();
+    check_rc(rc, "evict");
+    g_launches.fetch_add(2, std::memory_order_relaxed);
+    return THPVariable_Wrap(moved);
+}
+
+// verify_drafts(logits, tokens, seq_start, uniforms, temperature, draft_logits, draft_temperature, scratch) -> (keep, next)
+PyObject* verify_drafts_py(PyObject* const* args, Py_ssize_t n) {
+    if (n != 8) fail(PyExc_TypeError, "verify_drafts takes 8 arguments");
+    at::AutoDispatchBelowADInplaceOrView no_grad;
+    at::Tensor x = tensor(args[0]), near = optional_tensor(args[5]);
+    const at::Tensor tokens = tensor(args[1]), start = tensor(args[2]), uniforms = tensor(args[3]);
+    const double temperature = convert<double>(args[4]), near_temperature = args[6] == Py_None ? temperature : convert<double>(args[6]);
+    on_device(x, tokens, start, uniforms, near, args[7] == Py_None ? at::Tensor() : tensor(args[7]));
+    const auto rows = [](at::Tensor& t, const char* text) {
+        need(t.dim() == 2 && t.scalar_type() == at::kBFloat16 && t.size(0) >= 1 && t.size(0) <= 32767 && t.size(1) >= 1 && t.size(1) <= (1 << 20), text);
+        if (t.stride(1) != 1 || t.stride(0) < t.size(1)) t = t.contiguous();
+    };
+    rows(x, "verify_drafts: logits must be 1..32767 bf16 rows of 1..1048576 logits");
+    if (near.defined()) {
+        need(near.sizes() == x.sizes(), "verify_drafts: draft_logits must have the shape of logits");
+        rows(near, "verify_drafts: draft_logits must be bf16 rows");
+    }
+    const int64_t r = x.size(0), v = x.size(1);
+    need(tokens.dim() == 1 && tokens.size(0) == r && plain(tokens, at::kInt), "verify_drafts: tokens must be contiguous int32, one per row");
+    need(start.dim() == 1 && start.size(0) >= 2 && start.size(0) <= (1 << 24) && plain(start, at::kInt), "verify_drafts: seq_start must be contiguous int32 (S+1,)");
+    need(uniforms.dim() == 2 && uniforms.size(0) == r && uniforms.size(1) == 2 && (plain(uniforms, at::kFloat) || plain(uniforms, at::kDouble)),
+         "verify_drafts: uniforms must be contiguous float32 or float64 (R, 2)");
+    need(temperature > 0 && temperature < INFINITY && near_temperature > 0 && near_temperature < INFINITY,
+         "verify_drafts: temperatures must be positive and finite (greedy: sample_rows and accept_path)");
+    const int64_t s = start.size(0) - 1;
+    const c10::cuda::CUDAGuard on(x.device());
+    const auto stream = c10::cuda::getCurrentCUDAStream(x.device().index());
+    const at::Tensor scratch = buffer(args[7], tf_verify_scratch_bytes((int)r, (int)v), x);
+    const at::Tensor keep = at::empty({s}, tokens.options()), next = at::empty({s}, tokens.options());
+    const int rc = [&] {
+        const Released unlocked;
+        return tf_verify_rows(x.const_data_ptr(), (size_t)x.stride(0), data_of<void>(near), near.defined() ? (size_t)near.stride(0) : 0, data_of<int>(tokens),
+                              data_of<int>(start), uniforms.const_data_ptr(), uniforms.scalar_type() == at::kDouble, data_of<int>(keep), data_of<int>(next),
+                              scratch.mutable_data_ptr(), bytes_of(scratch), (int)r, (int)v, (int)s, temperature, near_temperature, stream.stream());
+    }();
+    check_rc(rc, "verify_drafts");
+    g_launches.fetch_add(2, std::memory_order_relaxed);
+    PyObject* pair = PyTuple_New(2);
+    if (pair == nullptr) throw PyErr{};
+    PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(keep));
+    PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(next));
+    return pair;
+}
+
 // current_stream(device index) -> cudaStream_t as an int; -1: the current device's
 PyObject* stream_py(PyObject* const* args, Py_ssize_t n) {
     const int dev = n > 0 ? convert<int>(args[0]) : -1;
@@ -305,6 +509,8 @@ PyMethodDef methods[] = {
     TF_FN(tf_window_slots, 0), TF_FN(tf_window_scratch_bytes, 0), TF_FN(tf_window_attention, 2), TF_FN(tf_attention_mass, 1),
     TF_FN(tf_evict_scratch_bytes, 0), TF_FN(tf_kv_evict, 2), TF_FN(tf_verify_scratch_bytes, 0), TF_FN(tf_verify_rows, 2),
     TF_OWN("bound", bound_py), TF_OWN("scratch", scratch_py), TF_OWN("lane_matmul", lane_matmul_py), TF_OWN("prefill_matmul", prefill_matmul_py),
+    TF_OWN("window_attention", window_attention_py), TF_OWN("attention_mass", attention_mass_py), TF_OWN("evict", evict_py),
+    TF_OWN("verify_drafts", verify_drafts_py),
     TF_OWN("current_stream", stream_py), TF_OWN("current_device", device_py), TF_OWN("launch_count", count_py),
     {nullptr, nullptr, 0, nullptr}};
 

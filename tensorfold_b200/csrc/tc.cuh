@@ -2,7 +2,7 @@
 // copies (TMA) for the kernels that use them.
 #pragma once
 
-#include <cuda.h>
+#include <cudaTypedefs.h>
 
 #include "common.cuh"
 
@@ -77,15 +77,31 @@ struct Waits {
     bool dead = false;
     __device__ explicit Waits(int* s) : status(s) {}
     __device__ void operator()(uint32_t bar, uint32_t parity) {
-        if (!dead && !mbar_wait(bar, parity, status, 1 << 16)) dead = true;
+        if (dead) return;
+        for (int i = 0; i < 64; ++i)
+            if (mbar_try_wait(bar, parity)) return;
+        dead = !mbar_wait_idle(bar, parity, status, 1000, 1 << 21);        // two seconds or so
     }
 };
-// D[tmem] (+)= A[smem descriptor] * B[smem descriptor]
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// Operand descriptors in two words. The low one holds the start address and the leading offset (in 16 bytes) and advances by constants,
+// the high one is the same for all operands here: next 8 rows 1024 bytes on, 128-byte swizzle. K-major operands ignore the leading
+// offset (1); for an MN-major one (V as the B operand: its rows are the contraction's index) it is the distance to the next 64 values.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t leading) { return (addr >> 4) | leading << 16; }
+// D[tmem] (+)= A[smem] * B[smem], issued where `leader`
+__device__ __forceinline__ void tc_mma_ss(bool leader, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
-        ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u)
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\tmov.b64 x, {%1, %7};\n\tmov.b64 y, {%2, %7};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, {%5, %5, %5, %5}, p;\n\t}"
+        ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(0u), "r"((uint32_t)leader), "n"(kDescHi)
+        : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem], issued where `leader`
+__device__ __forceinline__ void tc_mma_ts(bool leader, uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\tmov.b64 y, {%2, %7};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, {%5, %5, %5, %5}, p;\n\t}"
+        ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(0u), "r"((uint32_t)leader), "n"(kDescHi)
         : "memory");
 }
 __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -105,11 +121,6 @@ __device__ __forceinline__ void tc_dealloc(uint32_t tmem, uint32_t ncols) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(ncols) : "memory");
 }
 
-// MN-major operand with the 128-byte swizzle (V as the B operand: its rows are the contraction's index): atoms of 64 values x 8 rows,
-// 128 bytes a row, the next 8 rows 1024 bytes on (stride offset), the next 64 values `block` bytes on (leading offset).
-__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr, uint32_t block) {
-    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(block >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
 // kind::f16 instruction descriptor: fp32 sums, bf16 operands, M = 128
 __host__ __device__ constexpr uint32_t tc_idesc(int n, bool b_mn_major) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
@@ -133,6 +144,27 @@ __device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, int
 }
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
+// Descriptor of a tiled copy of rows of D values: (64 values, rows, outer, D / 64 slabs), or with the slabs before `outer`; a box is
+// box_rows rows of box_outer outer places and of one slab (K and Q, whose slabs lie apart in shared memory) or all of them (V).
+inline bool describe_rows(CUtensorMap* map, const void* base, int D, unsigned long long rows, size_t row_bytes, unsigned long long outer, size_t outer_bytes,
+              bool slabs_last, int box_rows, int box_outer, int box_slabs) {
+    static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult got;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &got) != cudaSuccess || got != cudaDriverEntryPointSuccess)
+            fn = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    }();
+    if (encode == nullptr) return false;
+    const int o = slabs_last ? 2 : 3, c = slabs_last ? 3 : 2;
+    cuuint64_t dims[4] = {64, rows, 0, 0}, strides[3] = {row_bytes, 0, 0};
+    cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 0, 0}, steps[4] = {1, 1, 1, 1};
+    dims[o] = outer; strides[o - 1] = outer_bytes; box[o] = (cuuint32_t)box_outer;
+    dims[c] = (cuuint64_t)(D / 64); strides[c - 1] = 128; box[c] = (cuuint32_t)box_slabs;
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace tf

@@ -19,8 +19,6 @@
 // NaN, rows that do not keep their bits. Every step of a row's arithmetic is fixed by its own position and keys and by the chunk
 // size, so a row alone, in a window and as a serial step has the same bits.
 
-#include <cudaTypedefs.h>
-
 #include "tc.cuh"
 
 namespace tf {
@@ -366,31 +364,31 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
         // ------------------------------- tensor-core issuer: Q K^T a tile ahead of P V ------------------------------------
         constexpr uint32_t qk_desc = tc_idesc(kTile, false), pv_desc = tc_idesc(D, true);
         const bool leader = elect_one();
-        const uint32_t qb = smem_u32(q_s);
+        // descriptors as low words that advance by constants; everything the loop depends on is uniform in the compiler's eyes, too: a
+        // product of 64 keys takes about as long as the moves into uniform registers that its operands would need otherwise
+        const uint32_t q_lo = desc_lo(smem_u32(q_s), 1);
         Ring kr(KS, 0), vr(VS, 0), qr(1, 0);
         int it = 0;                                      // tiles so far, over all items
         for (; item < a.items; item += gridDim.x) {
-            const Work w = work_of(a, item, raw, false);
+            const int tiles = __reduce_max_sync(0xffffffffu, work_of(a, item, raw, false).tiles);
             raw = fetch(a, item + gridDim.x);
-            if (w.tiles == 0) continue;
+            if (tiles == 0) continue;
             wait(q_full, qr.phase);
             qr.next();
-            for (int i = 0; i <= w.tiles; ++i) {
-                if (i < w.tiles) {
+            for (int i = 0; i <= tiles; ++i) {
+                if (i < tiles) {
                     const int t = it + i, b = t & 1;
                     wait(s_empty(b), (uint32_t)(((t >> 1) & 1) ^ 1));
                     wait(k_full(kr.i), kr.phase);
                     tc_fence_after();
-                    const uint32_t kb = smem_u32(k_s + kr.i * C::TILE_BYTES), d = tmem + C::S_COL + b * kTile;
+                    const uint32_t k_lo = desc_lo(smem_u32(k_s) + kr.i * C::TILE_BYTES, 1), d = tmem + C::S_COL + b * kTile;
 #pragma unroll
-                    for (int ks = 0; ks < D / 16; ++ks) {
-                        const uint64_t ad = smem_desc(qb + (ks >> 2) * C::Q_SLAB + (ks & 3) * 32), bd = smem_desc(kb + (ks >> 2) * C::K_SLAB + (ks & 3) * 32);
-                        if (leader) tc_mma_ss(d, ad, bd, qk_desc, ks > 0);
-                    }
+                    for (int ks = 0; ks < D / 16; ++ks)
+                        tc_mma_ss(leader, d, q_lo + (((ks >> 2) * C::Q_SLAB + (ks & 3) * 32) >> 4), k_lo + (((ks >> 2) * C::K_SLAB + (ks & 3) * 32) >> 4), qk_desc, ks > 0);
                     if (leader) {
                         tc_commit(s_full(b));
                         tc_commit(k_empty(kr.i));
-                        if (i + 1 == w.tiles) tc_commit(q_empty);
+                        if (i + 1 == tiles) tc_commit(q_empty);
                     }
                     kr.next();
                     __syncwarp();
@@ -400,18 +398,16 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
                     wait(v_full(vr.i), vr.phase);
                     wait(p_full(b), (uint32_t)((t >> 1) & 1));
                     tc_fence_after();
-                    const uint32_t vb = smem_u32(v_s + vr.i * C::TILE_BYTES);
+                    const uint32_t v_lo = desc_lo(smem_u32(v_s) + vr.i * C::TILE_BYTES, kPage * 128 / 16);
 #pragma unroll
-                    for (int pg = 0; pg < kTile / kPage; ++pg) {
-                        const uint64_t bd = smem_desc_mn(vb + pg * C::PAGE_BYTES, kPage * 128);
-                        if (leader) tc_mma_ts(tmem + C::O_COL, tmem + C::P_COL + b * (kTile / 2) + pg * 8, bd, pv_desc, i > 1 || pg > 0);
-                    }
+                    for (int pg = 0; pg < kTile / kPage; ++pg)
+                        tc_mma_ts(leader, tmem + C::O_COL, tmem + C::P_COL + b * (kTile / 2) + pg * 8, v_lo + pg * (C::PAGE_BYTES >> 4), pv_desc, i > 1 || pg > 0);
                     if (leader) { tc_commit(o_done(b)); tc_commit(v_empty(vr.i)); }
                     vr.next();
                     __syncwarp();
                 }
             }
-            it += w.tiles;
+            it += tiles;
         }
     } else {
         // ------------------------------- softmax: thread = query row ---------------------------------------------
@@ -636,27 +632,6 @@ __global__ void __launch_bounds__(128) window_join_kernel(const WindowArgs a) {
 }
 
 // ---- host side -----------------------------------------------------------------------------------------
-// Descriptor of a tiled copy of rows of D values: (64 values, rows, outer, D / 64 slabs), or with the slabs before `outer`; a box is
-// box_rows rows of box_outer outer places and of one slab (K and Q, whose slabs lie apart in shared memory) or all of them (V).
-bool describe(CUtensorMap* map, const void* base, int D, unsigned long long rows, size_t row_bytes, unsigned long long outer, size_t outer_bytes,
-              bool slabs_last, int box_rows, int box_outer, int box_slabs) {
-    static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
-        void* fn = nullptr;
-        cudaDriverEntryPointQueryResult got;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &got) != cudaSuccess || got != cudaDriverEntryPointSuccess)
-            fn = nullptr;
-        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-    }();
-    if (encode == nullptr) return false;
-    const int o = slabs_last ? 2 : 3, c = slabs_last ? 3 : 2;
-    cuuint64_t dims[4] = {64, rows, 0, 0}, strides[3] = {row_bytes, 0, 0};
-    cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 0, 0}, steps[4] = {1, 1, 1, 1};
-    dims[o] = outer; strides[o - 1] = outer_bytes; box[o] = (cuuint32_t)box_outer;
-    dims[c] = (cuuint64_t)(D / 64); strides[c - 1] = 128; box[c] = (cuuint32_t)box_slabs;
-    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int D, int QR>
 int launch_chunks(const WindowArgs& a, cudaStream_t st) {
     using C = Cfg<D, QR>;
@@ -674,10 +649,10 @@ int launch_chunks(const WindowArgs& a, cudaStream_t st) {
     const int G = a.H / a.HK;
     const unsigned long long H = a.H, HK = a.HK, R = a.R, rows = (unsigned long long)a.num_pages * HK * kPage;
     const size_t row = (size_t)D * 2;
-    if (!describe(&maps[0], a.q, D, H, row, R, row * H, true, G, a.group_rows, 1) ||
-        !describe(&maps[1], a.k_pages, D, rows, row, 1, row, false, kPage, 1, 1) || !describe(&maps[2], a.v_pages, D, rows, row, 1, row, false, kPage, 1, D / 64) ||
-        !describe(&maps[3], a.k_new, D, R < 16 ? 16 : R, row * HK, HK, row, false, kPage, 1, 1) ||
-        !describe(&maps[4], a.v_new, D, R < 16 ? 16 : R, row * HK, HK, row, false, kPage, 1, D / 64))
+    if (!describe_rows(&maps[0], a.q, D, H, row, R, row * H, true, G, a.group_rows, 1) ||
+        !describe_rows(&maps[1], a.k_pages, D, rows, row, 1, row, false, kPage, 1, 1) || !describe_rows(&maps[2], a.v_pages, D, rows, row, 1, row, false, kPage, 1, D / 64) ||
+        !describe_rows(&maps[3], a.k_new, D, R < 16 ? 16 : R, row * HK, HK, row, false, kPage, 1, 1) ||
+        !describe_rows(&maps[4], a.v_new, D, R < 16 ? 16 : R, row * HK, HK, row, false, kPage, 1, D / 64))
         return TF_ECUDA;
     void* args[] = {const_cast<WindowArgs*>(&a), &maps[0], &maps[1], &maps[2], &maps[3], &maps[4]};
     if (launch_pdl((const void*)window_chunk_kernel<D, QR>, dim3(a.items < kSms ? a.items : kSms), dim3(kThreads), C::SMEM, st, args) != cudaSuccess) {

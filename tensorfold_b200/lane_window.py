@@ -11,9 +11,6 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .lane_attention import PAGE
-
-TILE = 64
 
 
 def chunk_keys_for(n_seqs: int, heads: int, kv_heads: int, max_window: int, max_context: int, window: int | None = None, sinks: int = 0) -> int:
@@ -41,56 +38,20 @@ def window_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, 
     beside it, so an engine that compares windows with serial steps gives all its calls the same one.
     """
 
-    _lib.need_cuda(q, k_new, v_new, k_pages, v_pages, page_table, seq_lens, seq_start, lse, gate, out, scratch)
-    if q.dim() != 3 or k_new.dim() != 3 or k_pages.dim() != 4 or page_table.dim() != 2:
+    _lib.need_cuda(q)
+    if q.dim() != 3 or k_new.dim() != 3 or seq_lens.dim() != 1:
         raise ValueError("unsupported attention shape")
-    r, h, d = q.shape
-    hk = k_new.shape[1]
-    s = seq_lens.shape[0]
-    if (r < 1 or k_new.shape != (r, hk, d) or v_new.shape != k_new.shape or d not in (128, 256) or hk < 1 or h % hk or h // hk > 16
-            or k_pages.shape[1:] != (hk, PAGE, d) or v_pages.shape != k_pages.shape or page_table.shape[0] != s
-            or seq_start.shape != (s + 1,) or seq_lens.dim() != 1):
-        raise ValueError("unsupported attention shape")
-    for t in (q, k_new, v_new, k_pages, v_pages):
-        if t.dtype != torch.bfloat16 or not t.is_contiguous():
-            raise ValueError("attention tensors must be contiguous bf16")
-    for t in (page_table, seq_lens, seq_start):
-        if t.dtype != torch.int32 or not t.is_contiguous():
-            raise ValueError("page_table, seq_lens and seq_start must be contiguous int32")
-    if not 0 < scale < float("inf"):
-        raise ValueError("scale must be positive and finite")
-    if window is not None and window < 1 or sinks < 0 or max_window < 1 or max_context < max_window:
-        raise ValueError("window >= 1 (or None), sinks >= 0 and max_context >= max_window >= 1 required")
-    if chunk_keys is None:
-        chunk_keys = chunk_keys_for(s, h, hk, max_window, max_context, window, sinks)
-    if chunk_keys < TILE or chunk_keys % TILE:
-        raise ValueError(f"chunk_keys must be a positive multiple of {TILE}")
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (r, h) or not lse.is_contiguous()):
-        raise ValueError("lse must be contiguous float32 (R, H)")
-    if out is not None and (out.dtype != torch.bfloat16 or out.shape != q.shape or not out.is_contiguous()):
-        raise ValueError("out must be contiguous bf16 (R, H, D)")
-    if gate is not None and (gate.dtype != torch.bfloat16 or gate.shape != (r, h * 2 * d) or gate.stride(1) != 1):
-        raise ValueError("gate must be the (R, H * 2 * D) bf16 rows of the q projection")
-    if packed_out is not None and (packed_out.m != r or packed_out.k != h * d):
+    if packed_out is not None and (packed_out.m != q.shape[0] or packed_out.k != q.shape[1] * q.shape[2]):
         raise ValueError("packed_out must hold R rows of H * D inputs")
-    for t in (k_new, v_new, k_pages, v_pages, page_table, seq_lens, seq_start, lse, out, gate, scratch):
-        if t is not None and t.device != q.device:
-            raise ValueError("attention tensors must be on one device")
-    lib = _lib.load()
-    win = 0 if window is None else min(int(window), 1 << 30)
-    first = min(int(sinks), 1 << 30) if win else 0
-    need = lib.tf_window_scratch_bytes(r, h, d, lib.tf_window_slots(win, first, max_window, max_context, chunk_keys))
-    if scratch is None:
-        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
-    if out is None and packed_out is None:
-        out = torch.empty_like(q)
-    with _lib.on(q.device):
-        _lib.check(lib.tf_window_attention(
-            q, k_new, v_new, k_pages, v_pages, k_pages.shape[0], page_table, page_table.shape[1], seq_lens, seq_start, out, lse,
-            gate, gate.stride(0) if gate is not None else 0, packed_out.data if packed_out is not None else None,
-            packed_out.group if packed_out is not None else 64, scratch, scratch.numel() * scratch.element_size(), r, s, max_window,
-            max_context, win, first, chunk_keys, h, hk, d, float(scale), _lib.status(q.device).word, _lib.stream()), "window_attention")
-    return out if out is not None else packed_out
+    if window is not None and window < 1 or sinks < 0:
+        raise ValueError("window >= 1 (or None) and sinks >= 0 required")
+    if chunk_keys is None:
+        chunk_keys = chunk_keys_for(seq_lens.shape[0], q.shape[1], k_new.shape[1], max_window, max_context, window, sinks)
+    res = _lib.host().window_attention(q, k_new, v_new, k_pages, v_pages, page_table, seq_lens, seq_start, scale, max_window, max_context,
+                                       0 if window is None else min(window, 1 << 30), min(sinks, 1 << 30) if window is not None else 0, chunk_keys, scratch, out, lse, gate,
+                                       packed_out.data if packed_out is not None else None, packed_out.group if packed_out is not None else 64,
+                                       _lib.status(q.device).word)
+    return packed_out if res is None else res
 
 
 __all__ = ["chunk_keys_for", "window_attention"]

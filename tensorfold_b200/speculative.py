@@ -12,15 +12,6 @@ import torch
 
 from . import _lib
 
-MAX_VOCAB = 1 << 20
-
-
-def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
-    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape[0] < 1 or not 1 <= x.shape[1] <= MAX_VOCAB:
-        raise ValueError(f"verify_drafts: {what} must be bf16 rows of 1..{MAX_VOCAB} logits")
-    return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
-
-
 def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, seq_start: torch.Tensor, uniforms: torch.Tensor, *, temperature: float = 1.0,
                   draft_logits: torch.Tensor | None = None, draft_temperature: float | None = None, max_window: int | None = None,
                   scratch: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -37,36 +28,9 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, seq_start: torch.T
     least the longest window and may be left out. ``keep`` is what ``kv_commit`` and ``lane_evict.attention_mass`` take.
     """
 
-    _lib.need_cuda(logits, tokens, seq_start, uniforms, draft_logits, scratch)
-    x = _rows(logits, "logits")
-    r, v = x.shape
-    near = None if draft_logits is None else _rows(draft_logits, "draft_logits")
-    if near is not None and near.shape != x.shape:
-        raise ValueError("verify_drafts: draft_logits must have the shape of logits")
-    if tokens.shape != (r,) or tokens.dtype != torch.int32 or not tokens.is_contiguous():
-        raise ValueError("verify_drafts: tokens must be contiguous int32, one per row")
-    if seq_start.dim() != 1 or seq_start.shape[0] < 2 or seq_start.dtype != torch.int32 or not seq_start.is_contiguous():
-        raise ValueError("verify_drafts: seq_start must be contiguous int32 (S+1,)")
-    if uniforms.shape != (r, 2) or uniforms.dtype not in (torch.float32, torch.float64) or not uniforms.is_contiguous():
-        raise ValueError("verify_drafts: uniforms must be contiguous float32 or float64 (R, 2)")
-    near_t = temperature if draft_temperature is None else draft_temperature
-    if not 0 < temperature < float("inf") or not 0 < near_t < float("inf"):
-        raise ValueError("verify_drafts: temperatures must be positive and finite (greedy: sample_rows and accept_path)")
     if max_window is not None and max_window < 1:
         raise ValueError("verify_drafts: max_window must be positive")
-    if any(t is not None and t.device != logits.device for t in (tokens, seq_start, uniforms, near, scratch)):
-        raise ValueError("verify_drafts: tensors must be on one device")
-    s = seq_start.shape[0] - 1
-    lib = _lib.load()
-    need = lib.tf_verify_scratch_bytes(r, v)
-    if scratch is None:
-        scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
-    both = torch.empty((2, s), dtype=torch.int32, device=x.device)
-    with _lib.on(x.device):
-        _lib.check(lib.tf_verify_rows(x, x.stride(0), near, near.stride(0) if near is not None else 0, tokens, seq_start, uniforms,
-                                      int(uniforms.dtype == torch.float64), both[0], both[1], scratch, scratch.numel() * scratch.element_size(),
-                                      r, v, s, float(temperature), float(near_t), _lib.stream()), "verify_drafts")
-    return both[0], both[1]
+    return _lib.host().verify_drafts(logits, tokens, seq_start, uniforms, temperature, draft_logits, draft_temperature, scratch)
 
 
-__all__ = ["MAX_VOCAB", "verify_drafts"]
+__all__ = ["verify_drafts"]
