@@ -9,7 +9,7 @@
 // move into the evicted ones below it, in order (keys carry their rotation, so their order does not matter): a slot that
 // stays below the budget is not touched, and the fewest possible rows travel.
 
-#include "common.cuh"
+#include "tc.cuh"
 
 namespace tf {
 namespace {
@@ -29,38 +29,197 @@ struct MassArgs {
     float scale_log2;
 };
 
-// First form: a block per (page, KV head, layer and sequence), a warp per four keys, rows one by one.
+// S^T = K Q^T on the tensor core: a tile of 128 keys is the A operand (its rows the tensor memory's lanes), the kept query rows, up to 128 at a
+// time, the B operand, so that a key's scores lie in one thread's lane and its sum needs no shuffle and no atomic: thread = key, columns
+// in row order, fp32. K arrives a page at a time by tiled copies; slots behind the last key are never added.
+//
+// A block walks the tiles of one (layer, sequence, KV head) that are its share, the row chunks inner: with up to 128 rows (the usual
+// case) Q is staged once. What bounds it: the bytes of K, and 2^x on the special-function units (16 a cycle and SM): a tile's 128 x 48 weights
+// take 400 cycles, its 64 KB 1.5 us at the SM's share of the memory's rate.
+constexpr int kMassKeys = 128, kMassRows = 128, kMassSum = 4, kMassMma = 4, kMassLoad = 5, kMassThreads = 6 * 32;
+
 template <int D>
-__global__ void __launch_bounds__(128) mass_kernel(const MassArgs a) {
-    constexpr int PER = D / 32;
+struct MassCfg {
+    static constexpr int SLABS = D / 64, K_SLAB = kMassKeys * 128, TILE_BYTES = SLABS * K_SLAB, Q_SLAB = kMassRows * 128, Q_BYTES = SLABS * Q_SLAB;
+    static constexpr int KS = D == 256 ? 2 : 4;
+    static constexpr int NBARS = 2 * KS + 4 + 2;
+    static constexpr int SMEM = Q_BYTES + KS * TILE_BYTES + kMassRows * 4 + NBARS * 8 + 1024;
+    static_assert(SMEM <= 227 * 1024, "shared memory");
+};
+
+template <int D>
+__global__ void __launch_bounds__(kMassThreads, 1) mass_kernel(const __grid_constant__ MassArgs a, const __grid_constant__ CUtensorMap k_map) {
+    using C = MassCfg<D>;
+    constexpr int KS = C::KS, CPR = D / 8;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint32_t tmem_s;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint8_t* q_s = smem + ((1024u - (smem_u32(smem) & 1023u)) & 1023u);
+    uint8_t* k_s = q_s + C::Q_BYTES;
+    float* lse_s = reinterpret_cast<float*>(k_s + KS * C::TILE_BYTES);               // of the staged rows, log2 domain
+    const uint32_t bars = smem_u32(lse_s + kMassRows);
+    auto k_full = [&](int s) { return bars + 8u * s; };
+    auto k_empty = [&](int s) { return bars + 8u * (KS + s); };
+    auto s_full = [&](int s) { return bars + 8u * (2 * KS + s); };
+    auto s_empty = [&](int s) { return bars + 8u * (2 * KS + 2 + s); };
+    const uint32_t q_full = bars + 8u * (2 * KS + 4), q_empty = q_full + 8;
     pdl_launch_dependents();
     pdl_wait();
-    const int kvh = blockIdx.y, layer = blockIdx.z / a.S, seq = blockIdx.z % a.S, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int r0 = a.seq_start[seq], n = a.seq_start[seq + 1] - r0, L = a.seq_lens[seq], kept = min(max(a.keep[seq], 0), n);
-    if (L + kept > a.max_context && threadIdx.x == 0) report(a.status, TF_EINVAL);
-    const int j0 = blockIdx.x * kPage, end = min(L + kept, min(a.max_context, a.max_pages * kPage));
-    if (kept == 0 || j0 >= end) return;
-    const int page = a.page_table[(size_t)seq * a.max_pages + blockIdx.x];
-    if (page < 0 || page >= a.num_pages) { report(a.status, TF_EINVAL); return; }
-    const int G = a.H / a.HK;
-    const size_t cell0 = (((size_t)layer * a.num_pages + page) * a.HK + kvh) * kPage;
-    for (int jj = warp; jj < kPage && j0 + jj < end; jj += 4) {
-        const int j = j0 + jj;
-        float k[PER], sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) k[i] = bf2f(a.k_pages[(cell0 + jj) * D + lane * PER + i]);
-        for (int t = max(0, j - L); t < kept; ++t)
-            for (int g = 0; g < G; ++g) {
-                const size_t row = ((size_t)layer * a.R + r0 + t) * a.H + kvh * G + g;
-                float s = 0.f;
-#pragma unroll
-                for (int i = 0; i < PER; ++i) s = fmaf(k[i], bf2f(a.q[row * D + lane * PER + i]), s);
-                sum += exp2f(warp_sum(s) * a.scale_log2 - a.lse[row] * kLog2e);
+    // ---- the block's share of the tiles of (layer, sequence, KV head) ----
+    const int kvh = blockIdx.y, layer = blockIdx.z / a.S, seq = blockIdx.z - layer * a.S, G = a.H / a.HK;
+    const int r0 = a.seq_start[seq], n = a.seq_start[seq + 1] - r0, L = a.seq_lens[seq];
+    int kept = min(max(a.keep[seq], 0), n);
+    if (kept < 1) return;
+    if (r0 < 0 || r0 + n > a.R || L < 0 || L > a.max_context - kept || L > a.max_pages * kPage - kept) {      // not what the call was made for
+        if (tid == 0) report(a.status, TF_EINVAL);
+        return;
+    }
+    const int keys = L + kept, tiles = (keys + kMassKeys - 1) / kMassKeys;
+    const int per = (tiles + gridDim.x - 1) / gridDim.x, first = blockIdx.x * per, last = min(tiles, first + per);
+    if (first >= last) return;
+    const int rows = kept * G, chunks = (rows + kMassRows - 1) / kMassRows;
+    if (tid == 0) {
+        for (int s = 0; s < KS; ++s) { mbar_init(k_full(s), 1); mbar_init(k_empty(s), 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(s_full(s), 1); mbar_init(s_empty(s), kMassSum); }
+        mbar_init(q_full, kMassSum);
+        mbar_init(q_empty, 1);
+        mbar_fence_init();
+    }
+    if (warp == kMassMma) tc_alloc(smem_u32(&tmem_s), 2 * kMassRows);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_s;
+    Waits wait(a.status);
+
+    if (warp == kMassLoad) {
+        const int* pt = a.page_table + (size_t)seq * a.max_pages;
+        Ring ring(KS, 1);
+        for (int t = first; t < last; ++t) {
+            // eight pages, a lane each; one behind the last key or that is none (reported) is copied from page 0 and not used
+            int page = 0;
+            const int j = t * kMassKeys + lane * kPage;
+            if (lane < 8 && j < keys) {
+                page = pt[j / kPage];
+                if (page < 0 || page >= a.num_pages) { report(a.status, TF_EINVAL); page = 0; }
             }
-        if (lane == 0) {
-            a.mass[cell0 + jj] = j < L ? a.mass[cell0 + jj] + sum : sum;
-            if (j >= L) a.pos[cell0 + jj] = a.row_pos[r0 + j - L];
+            wait(k_empty(ring.i), ring.phase);
+            if (lane == 0) mbar_arrive_expect_tx(k_full(ring.i), C::TILE_BYTES);
+            __syncwarp();
+            if (lane < 8) {
+                const int y = ((layer * a.num_pages + page) * a.HK + kvh) * kPage;
+                const uint32_t to = smem_u32(k_s) + ring.i * C::TILE_BYTES + lane * (kPage * 128);
+#pragma unroll
+                for (int c = 0; c < C::SLABS; ++c) tma_4d(to + c * C::K_SLAB, &k_map, 0, y, c, 0, k_full(ring.i));
+            }
+            __syncwarp();
+            ring.next();
         }
+    } else if (warp == kMassMma) {
+        const bool leader = elect_one();
+        const uint32_t q_lo = desc_lo(smem_u32(q_s), 1);
+        Ring kr(KS, 0), qr(1, 0), sr(2, 1);
+        const int mine = __reduce_max_sync(0xffffffffu, last - first), parts = __reduce_max_sync(0xffffffffu, chunks);
+        const int least = __reduce_max_sync(0xffffffffu, rows);
+        for (int t = 0; t < mine; ++t) {
+            wait(k_full(kr.i), kr.phase);
+            const uint32_t k_lo = desc_lo(smem_u32(k_s) + kr.i * C::TILE_BYTES, 1);
+            for (int c = 0; c < parts; ++c) {
+                if (parts > 1 || t == 0) {
+                    wait(q_full, qr.phase);
+                    qr.next();
+                }
+                wait(s_empty(sr.i), sr.phase);
+                tc_fence_after();
+                // columns in sixteens (N of the tensor core with M = 128)
+                const uint32_t idesc = tc_idesc((min(kMassRows, least - c * kMassRows) + 15) & ~15, false);
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks)
+                    tc_mma_ss(leader, tmem + sr.i * kMassRows, k_lo + (((ks >> 2) * C::K_SLAB + (ks & 3) * 32) >> 4), q_lo + (((ks >> 2) * C::Q_SLAB + (ks & 3) * 32) >> 4), idesc,
+                              ks > 0);
+                if (leader) {
+                    tc_commit(s_full(sr.i));
+                    if (parts > 1) tc_commit(q_empty);
+                    if (c + 1 == parts) tc_commit(k_empty(kr.i));
+                }
+                __syncwarp();
+                sr.next();
+            }
+            kr.next();
+        }
+    } else {
+        const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+        const size_t plane = (size_t)layer * a.num_pages * a.HK * kPage;
+        const int* pt = a.page_table + (size_t)seq * a.max_pages;
+        Ring sr(2, 0), qr(1, 1);
+        auto stage = [&](int c) {            // rows c * 128 ..: into shared memory, with their log-sum-exps
+            const int q0 = c * kMassRows, count = min(kMassRows, rows - q0);
+            const size_t row0 = (size_t)layer * a.R + r0;
+            for (int e = tid; e < count * CPR; e += kMassSum * 32) {
+                const int r = e / CPR, x = e % CPR, t = (q0 + r) / G;
+                const uint4 v = *reinterpret_cast<const uint4*>(a.q + ((row0 + t) * a.H + kvh * G + q0 + r - t * G) * D + x * 8);
+                *reinterpret_cast<uint4*>(q_s + (x >> 3) * C::Q_SLAB + r * 128 + (((x ^ r) & 7) << 4)) = v;
+            }
+            if (tid < count) {
+                const int t = (q0 + tid) / G;
+                lse_s[tid] = a.lse[(row0 + t) * a.H + kvh * G + q0 + tid - t * G] * kLog2e;
+            }
+            named_bar_sync(1, kMassSum * 32);            // the log-sum-exps are everybody's
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        };
+        if (chunks == 1) stage(0);
+        for (int t = first; t < last; ++t) {
+            const int j = t * kMassKeys + tid;
+            float sum = 0.f;
+            // the key's old weight, under way while the scores are formed
+            size_t cell = 0;
+            float old = 0.f;
+            bool real = j < keys;
+            if (real) {
+                const int page = pt[j / kPage];
+                real = page >= 0 && page < a.num_pages;
+                cell = plane + ((size_t)(real ? page : 0) * a.HK + kvh) * kPage + j % kPage;
+                if (real && j < L) old = a.mass[cell];
+            }
+            const int from = max(0, j - L) * G;          // rows that come before the key itself
+            for (int c = 0; c < chunks; ++c) {
+                if (chunks > 1) {
+                    wait(q_empty, qr.phase);             // the products of the rows before have read them ...
+                    qr.next();
+                    named_bar_sync(1, kMassSum * 32);    // ... and so have the sums
+                    stage(c);
+                }
+                wait(s_full(sr.i), sr.phase);
+                tc_fence_after();
+                const int q0 = c * kMassRows, count = min(kMassRows, rows - q0);
+                for (int x = 0; x < count; x += 16) {
+                    float s[16];
+                    tc_ld16(lanes + sr.i * kMassRows + x, s);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float p = fast_exp2(fmaf(s[e], a.scale_log2, -lse_s[x + e]));
+                        sum += x + e < count && q0 + x + e >= from ? p : 0.f;
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_empty(sr.i));
+                sr.next();
+            }
+            if (real) {
+                a.mass[cell] = old + sum;
+                if (j >= L) a.pos[cell] = a.row_pos[r0 + j - L];
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMassMma) {
+        tc_fence_after();
+        tc_dealloc(tmem, 2 * kMassRows);
     }
 }
 
@@ -220,6 +379,34 @@ __global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const Evict
     }
 }
 
+constexpr int kSms = 148;
+
+template <int D>
+int launch_mass(const MassArgs& a, int layers, cudaStream_t st) {
+    using C = MassCfg<D>;
+    static bool configured[64] = {};       // the opt-in is per device
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return TF_ECUDA; }
+    if (!configured[dev]) {
+        if (cudaFuncSetAttribute(mass_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) {
+            cudaGetLastError();
+            return TF_ECUDA;
+        }
+        configured[dev] = true;
+    }
+    CUtensorMap map;
+    if (!describe_rows(&map, a.k_pages, D, (unsigned long long)layers * a.num_pages * a.HK * kPage, (size_t)D * 2, 1, (size_t)D * 2, false, kPage, 1, 1)) return TF_ECUDA;
+    // blocks a column (layer, sequence, KV head): several rounds of the SMs, so that columns of unequal length even out
+    const long long columns = (long long)layers * a.S * a.HK, tiles = (a.max_context + kMassKeys - 1) / kMassKeys;
+    const long long wanted = (4ll * kSms + columns - 1) / columns, blocks = wanted < tiles ? wanted : tiles;
+    void* args[] = {const_cast<MassArgs*>(&a), &map};
+    if (launch_pdl((const void*)mass_kernel<D>, dim3((unsigned)blocks, a.HK, layers * a.S), dim3(kMassThreads), C::SMEM, st, args) != cudaSuccess) {
+        cudaGetLastError();
+        return TF_ECUDA;
+    }
+    return TF_OK;
+}
+
 }  // namespace
 }  // namespace tf
 
@@ -234,14 +421,10 @@ int tf_attention_mass(const void* q, const float* lse, const void* k_pages, int 
         return TF_EINVAL;
     if (!q || !lse || !k_pages || !page_table || !seq_lens || !seq_start || !keep || !row_pos || !mass || !pos) return TF_EINVAL;
     if (((uintptr_t)q | (uintptr_t)k_pages) & 15 || ((uintptr_t)mass | (uintptr_t)pos | (uintptr_t)lse) & 3) return TF_EALIGN;
-    if ((long long)layers * n_seqs > 65535 || kv_heads > 65535) return TF_EINVAL;
+    if ((long long)layers * n_seqs > 65535 || kv_heads > 65535 || (long long)layers * num_pages * kv_heads * 16 > 0x7FFFFFFFll) return TF_EINVAL;
     tf::MassArgs a{static_cast<const __nv_bfloat16*>(q), lse, static_cast<const __nv_bfloat16*>(k_pages), page_table, seq_lens, seq_start, keep,
                    row_pos, mass, pos, status, num_pages, max_pages, heads, kv_heads, rows, n_seqs, max_context, scale * tf::kLog2e};
-    void* args[] = {&a};
-    const void* kern = head_dim == 256 ? (const void*)tf::mass_kernel<256> : (const void*)tf::mass_kernel<128>;
-    if (tf::launch_pdl(kern, dim3((max_context + tf::kPage - 1) / tf::kPage, kv_heads, layers * n_seqs), dim3(128), 0, static_cast<cudaStream_t>(stream),
-                       args) != cudaSuccess) { cudaGetLastError(); return TF_ECUDA; }
-    return TF_OK;
+    return head_dim == 256 ? tf::launch_mass<256>(a, layers, static_cast<cudaStream_t>(stream)) : tf::launch_mass<128>(a, layers, static_cast<cudaStream_t>(stream));
 }
 
 size_t tf_evict_scratch_bytes(int layers, int n_seqs, int kv_heads, int budget, int max_context) {
