@@ -458,8 +458,8 @@ PyObject* verify_drafts_py(PyObject* const* args, Py_ssize_t n) {
     need(start.dim() == 1 && start.size(0) >= 2 && start.size(0) <= (1 << 24) && plain(start, at::kInt), "verify_drafts: seq_start must be contiguous int32 (S+1,)");
     need(uniforms.dim() == 2 && uniforms.size(0) == r && uniforms.size(1) == 2 && (plain(uniforms, at::kFloat) || plain(uniforms, at::kDouble)),
          "verify_drafts: uniforms must be contiguous float32 or float64 (R, 2)");
-    need(temperature > 0 && temperature < INFINITY && near_temperature > 0 && near_temperature < INFINITY,
-         "verify_drafts: temperatures must be positive and finite (greedy: sample_rows and accept_path)");
+    need(temperature >= 1e-6 && temperature <= 1e6 && near_temperature >= 1e-6 && near_temperature <= 1e6,
+         "verify_drafts: temperatures must be in 1e-6..1e6 (greedy: sample_rows and accept_path)");
     const int64_t s = start.size(0) - 1;
     const c10::cuda::CUDAGuard on(x.device());
     const auto stream = c10::cuda::getCurrentCUDAStream(x.device().index());

@@ -126,6 +126,23 @@ __host__ __device__ constexpr uint32_t tc_idesc(int n, bool b_mn_major) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
 
+// two fp32 values in one register pair: one instruction on both
+__device__ __forceinline__ unsigned long long pair_of(float x, float y) {
+    unsigned long long v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    return v;
+}
+__device__ __forceinline__ void split_pair(unsigned long long v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ unsigned long long fma_pair(unsigned long long x, unsigned long long y, unsigned long long z) {
+    unsigned long long v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(x), "l"(y), "l"(z));
+    return v;
+}
+__device__ __forceinline__ unsigned long long add_pair(unsigned long long x, unsigned long long y) {
+    unsigned long long v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
+    return v;
+}
 // 2^x on the special-function unit, denormals flushed
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;

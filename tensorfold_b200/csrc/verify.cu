@@ -9,16 +9,18 @@
 //
 // The draw is the first token in vocabulary order whose cumulative weight is above u2 times the total.
 //
-// Two launches. Row statistics: a slice of 8192 logits a block, its maximum and the sum of 2^((x - max) log2e / T) - bound by the
-// bytes of the logits. Choice: a cluster of blocks per sequence; every block forms the acceptances from the slices' sums (64 bits), then the cluster
-// goes over the one row that is drawn from. An acceptance is one comparison, so 32-bit exponentials (relative error of
-// p and q near 3e-7) decide all but one in some million draws as exact arithmetic would; a draw compares one
-// number with up to a million borders, so its weights and sums are in 64 bits throughout. A NaN logit counts as -inf and +inf as the
-// largest bf16 value.
+// Two launches. Row statistics: a slice of 8192 logits a block, with y = logit * log2e / T an offset o near its largest y and the sum of
+// 2^(y - o) - bound by the bytes of the logits (128 + 112 rows of 248320: @STATS@). Choice: a cluster of eight blocks per sequence; every block
+// forms the acceptances from the slices' sums (64 bits), then the cluster goes over the one row that is drawn from, twice where
+// a drafter's distribution has to be normalised too - bound by the 64-bit pipe (16 rows of 248320 with a drafter: @CHOICE@, of which two thirds are its ten
+// instructions a weight). An acceptance is one comparison, so 32-bit exponentials (relative error of p and q near 1e-6) decide
+// all but one in a million draws as exact arithmetic would; a draw compares one number with up to a million borders, so its
+// weights and sums are in 64 bits throughout. A NaN logit counts as -inf, +inf as a very
+// large one (tame).
 
 #include <cooperative_groups.h>
 
-#include "common.cuh"
+#include "tc.cuh"
 
 namespace tf {
 namespace {
@@ -26,9 +28,11 @@ namespace cg = cooperative_groups;
 
 constexpr int kStatThreads = 256, kStatChunks = 4;                  // chunks of 8 logits a thread
 constexpr int kSlice = kStatThreads * kStatChunks * 8;              // logits a slice
-constexpr int kChoiceThreads = 512, kCluster = 8, kChoiceWarps = kChoiceThreads / 32;
+constexpr int kChoiceThreads = 1024, kCluster = 8, kChoiceWarps = kChoiceThreads / 32;
+constexpr int kKept = 128;                                          // window rows whose offsets are kept between the two steps
 constexpr int kSegment = 256;                                       // logits a warp takes at a time
 constexpr int kMaxVocab = 1 << 20;
+constexpr uint32_t kNone = 0xFF80FF80u;                              // two bf16 -inf
 constexpr int kMaxSegments = kMaxVocab / kCluster / kSegment + 2;
 
 struct VerifyArgs {
@@ -39,36 +43,48 @@ struct VerifyArgs {
     int *keep, *next;
     float2* stats;                            // [2 (target, draft)][R][slices]: maximum, sum
     int V, R, S, slices, u64;
-    float c, draft_c;                         // log2e / temperature
-    double inv, draft_inv;                    // 1 / temperature
+    float c, draft_c, most, draft_most;       // log2e / temperature; the largest logit (see tame)
+    double c64, draft_c64;
 };
 
-__device__ __forceinline__ float tame(float x) {       // NaN -> -inf, +inf -> the largest bf16
-    return x != x ? -INFINITY : fminf(x, 3.3895313892515355e38f);
-}
+// NaN -> -inf; more than `most` -> `most`: logit / temperature up to 7e8, where an offset in 32 bits still leaves 2^(y - offset) in range
+__device__ __forceinline__ float tame(float x, float most) { return x != x ? -INFINITY : fminf(x, most); }
 
 // A row seen as chunks of eight logits on 16-byte boundaries: chunk c holds logits 8c - skew .. 8c - skew + 7, those that exist.
 struct Row {
     const __nv_bfloat16* p;
     int skew, V;
-    __device__ Row(const __nv_bfloat16* row, int V_) : p(row), skew((int)((reinterpret_cast<uintptr_t>(row) & 15) >> 1)), V(V_) {}
+    float most;
+    __device__ Row(const __nv_bfloat16* row, int V_, float most_) : p(row), skew((int)((reinterpret_cast<uintptr_t>(row) & 15) >> 1)), V(V_), most(most_) {}
     __device__ int chunks() const { return (V + skew + 7) >> 3; }
     __device__ int first(int c) const { return 8 * c - skew; }
-    __device__ void load(int c, float (&x)[8]) const {
+    __device__ uint4 raw(int c) const {          // -inf where there is none
         const int i = first(c);
-        if (i >= 0 && i + 8 <= V) {
-            unpack8(*reinterpret_cast<const uint4*>(p + i), x);
+        if (i >= 0 && i + 8 <= V) return *reinterpret_cast<const uint4*>(p + i);
+        uint32_t u[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = tame(x[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = i + e >= 0 && i + e < V ? tame(bf2f(p[i + e])) : -INFINITY;
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t lo = i + 2 * e >= 0 && i + 2 * e < V ? __bfloat16_as_ushort(p[i + 2 * e]) : kNone & 0xFFFFu;
+            const uint32_t hi = i + 2 * e + 1 >= 0 && i + 2 * e + 1 < V ? __bfloat16_as_ushort(p[i + 2 * e + 1]) : kNone & 0xFFFFu;
+            u[e] = lo | hi << 16;
         }
+        return make_uint4(u[0], u[1], u[2], u[3]);
+    }
+    __device__ void load(int c, float (&x)[8]) const {
+        unpack8(raw(c), x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = tame(x[e], most);
     }
 };
 
+// the larger of two bf16 pairs, a NaN losing to any number
+__device__ __forceinline__ uint32_t max_pair(uint32_t x, uint32_t y) {
+    const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
+    return *reinterpret_cast<const uint32_t*>(&m);
+}
+
 __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const VerifyArgs a) {
-    __shared__ float red[kStatThreads / 32];
+    __shared__ float red[2][kStatThreads / 32];
     pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -76,105 +92,148 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
     const int row = blockIdx.y - (drafter ? a.R : 0);
     // rows behind the last sequence are nobody's, a first row was not drafted
     bool skip = row >= a.seq_start[a.S];
-    if (drafter)
+    if (drafter) {
         for (int s = tid; s < a.S; s += kStatThreads) skip |= a.seq_start[s] == row;
-    if (__syncthreads_or(skip)) return;
-    const Row r(drafter ? a.draft + (size_t)row * a.draft_stride : a.logits + (size_t)row * a.stride, a.V);
+        if (__syncthreads_or(skip)) return;
+    }
+    const Row r(drafter ? a.draft + (size_t)row * a.draft_stride : a.logits + (size_t)row * a.stride, a.V,
+                drafter ? a.draft_most : a.most);
     const float c = drafter ? a.draft_c : a.c;
     const int chunks = r.chunks(), c0 = blockIdx.x * (kSlice / 8) + tid;
-    float x[kStatChunks][8], m = -INFINITY;
+    uint4 v[kStatChunks];
 #pragma unroll
-    for (int k = 0; k < kStatChunks; ++k) {
-        if (c0 + k * kStatThreads < chunks) {
-            r.load(c0 + k * kStatThreads, x[k]);
-        } else {
+    for (int k = 0; k < kStatChunks; ++k) v[k] = c0 + k * kStatThreads < chunks ? r.raw(c0 + k * kStatThreads) : make_uint4(kNone, kNone, kNone, kNone);
+    if (skip) return;                            // the whole block, where it is not a drafter's
+    uint32_t m2 = kNone;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[k][e] = -INFINITY;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) m = fmaxf(m, x[k][e]);
-    }
-    m = warp_max(m);
-    if (lane == 0) red[warp] = m;
+    for (int k = 0; k < kStatChunks; ++k) m2 = max_pair(max_pair(m2, max_pair(v[k].x, v[k].y)), max_pair(v[k].z, v[k].w));
+    float m = warp_max(fmaxf(bf16_lo(m2), bf16_hi(m2)));
+    if (lane == 0) red[0][warp] = m;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kStatThreads / 32; ++w) m = fmaxf(m, red[w]);
-    __syncthreads();
+    for (int w = 0; w < kStatThreads / 32; ++w) m = fmaxf(m, red[0][w]);
+    const float o = fminf(m, r.most) * c;
     float s = 0.f;
-    if (m > -INFINITY) {
+    if (o > -INFINITY) {
+        const unsigned long long c2 = pair_of(c, c), o2 = pair_of(-o, -o);
+        unsigned long long sum[2] = {0, 0};              // two zeros each
 #pragma unroll
-        for (int k = 0; k < kStatChunks; ++k)
+        for (int k = 0; k < kStatChunks; ++k) {
+            const uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s += exp2f((x[k][e] - m) * c);
+            for (int e = 0; e < 4; ++e) {
+                float x, y;
+                split_pair(fma_pair(pair_of(bf16_lo(u[e]), bf16_hi(u[e])), c2, o2), x, y);
+                sum[e & 1] = add_pair(sum[e & 1], pair_of(fast_exp2(x), fast_exp2(y)));
+            }
+        }
+        float x, y;
+        split_pair(add_pair(sum[0], sum[1]), x, y);
+        s = x + y;
     }
     s = warp_sum(s);
-    if (lane == 0) red[warp] = s;
+    if (lane == 0) red[1][warp] = s;
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < kStatThreads / 32; ++w) s += red[w];
-        a.stats[(size_t)blockIdx.y * a.slices + blockIdx.x] = make_float2(m, s);
+    s = red[1][0];
+#pragma unroll
+    for (int w = 1; w < kStatThreads / 32; ++w) s += red[1][w];
+    if (!(s < INFINITY)) {                       // a NaN or +inf among the logits: again, one by one
+        s = 0.f;
+#pragma unroll 1
+        for (int k = 0; k < kStatChunks; ++k) {
+            float x[8];
+            if (c0 + k * kStatThreads < chunks) r.load(c0 + k * kStatThreads, x);
+            for (int e = 0; e < 8; ++e) s += c0 + k * kStatThreads < chunks && x[e] > -INFINITY ? fast_exp2(fmaf(x[e], c, -o)) : 0.f;
+        }
+        s = warp_sum(s);
+        __syncthreads();
+        if (lane == 0) red[1][warp] = s;
+        __syncthreads();
+        s = red[1][0];
+        for (int w = 1; w < kStatThreads / 32; ++w) s += red[1][w];
     }
+    if (tid == 0) a.stats[(size_t)blockIdx.y * a.slices + blockIdx.x] = make_float2(o, s);
 }
 
-// A row's maximum and sum from its slices, in 64 bits. Whole warps.
-__device__ __forceinline__ void row_stats(const float2* st, int slices, double inv, float& m, double& z) {
-    const int lane = threadIdx.x & 31;
-    m = -INFINITY;
-    for (int i = lane; i < slices; i += 32) m = fmaxf(m, st[i].x);
-    m = warp_max(m);
-    z = 0.0;
-    if (m > -INFINITY)
-        for (int i = lane; i < slices; i += 32)
-            if (st[i].x > -INFINITY) z += st[i].y * exp(((double)st[i].x - m) * inv);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-}
+// 2^t for t < 1000 in 64 bits: t = n / 64 + r, a table of 2^(j/64), and the series of 2^r = e^(r ln 2) to the fifth power (|r| <= 1/128: the
+// next term is 4e-17). Zero below 2^-1000.
+struct Exp2 {
+    const double* table;                         // shared memory
+    __device__ double operator()(double t) const {
+        constexpr double l = 0.69314718055994530942;
+        const double shifter = 6755399441055744.0;                     // 1.5 * 2^52: adding it leaves the nearest integer in the low word
+        const double big = fma(t, 64.0, shifter);
+        const int n = __double2loint(big);
+        const double r = fma(big - shifter, -1.0 / 64.0, t);
+        double y = fma(r, l * l * l * l * l / 120, l * l * l * l / 24);
+        y = fma(r, y, l * l * l / 6);
+        y = fma(r, y, l * l / 2);
+        y = fma(r, y, l);
+        y = fma(r, y, 1.0);
+        const double p = table[n & 63];
+        const double scaled = __hiloint2double(__double2hiint(p) + ((n >> 6) << 20), __double2loint(p));
+        return t > -1000.0 ? y * scaled : 0.0;
+    }
+};
 
-__device__ __forceinline__ double block_sum(double v, double* warp_s) {     // every thread gets it
+// A row's offset and sum from its slices. Whole warps.
+__device__ __forceinline__ float row_offset(const float2* st, int slices) {
+    float o = -INFINITY;
+    for (int i = threadIdx.x & 31; i < slices; i += 32) o = fmaxf(o, st[i].x);
+    return warp_max(o);
+}
+__device__ __forceinline__ double row_sum(const float2* st, int slices, float o, const Exp2& exp2_64) {
+    double z = 0.0;
+    for (int i = threadIdx.x & 31; i < slices; i += 32)
+        if (st[i].x > -INFINITY) z += st[i].y * exp2_64((double)st[i].x - o);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) warp_s[threadIdx.x >> 5] = v;
-    __syncthreads();
-    double s = 0.0;
-    for (int w = 0; w < kChoiceWarps; ++w) s += warp_s[w];
-    return s;
+    for (int k = 16; k; k >>= 1) z += __shfl_xor_sync(0xffffffffu, z, k);
+    return z;
 }
 
 enum Weights { kAll, kWithout, kResidual };     // p; p without the draft; max(p - q, 0)
 
-__global__ void __launch_bounds__(kChoiceThreads) verify_choice_kernel(const VerifyArgs a) {
-    __shared__ double warp_s[kChoiceWarps], seg[kMaxSegments], cum[kMaxSegments], share[4];
+__global__ void __launch_bounds__(kChoiceThreads, 1) verify_choice_kernel(const VerifyArgs a) {
+    __shared__ double table[64], part[2][kChoiceWarps], seg[kMaxSegments], cum[kMaxSegments], share[4];
+    __shared__ float offset_s[2][kKept];         // target's and drafter's, of the window's first rows
     __shared__ int first_out;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid < 64) table[tid] = exp2(tid / 64.0);
     pdl_launch_dependents();
     pdl_wait();
-    cg::cluster_group cluster = cg::this_cluster();
     const int seq = blockIdx.x / kCluster, rank = blockIdx.x % kCluster;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int r0 = a.seq_start[seq], n = a.seq_start[seq + 1] - r0;
     if (n < 1) {                                 // a sequence without rows: the whole cluster leaves
         if (rank == 0 && tid == 0) { a.keep[seq] = 0; a.next[seq] = -1; }
         return;
     }
+    const Exp2 exp2_64{table};
     auto uniform = [&](int row, int i) -> double {
         return a.u64 ? static_cast<const double*>(a.uniforms)[2 * (size_t)row + i] : (double)static_cast<const float*>(a.uniforms)[2 * (size_t)row + i];
     };
     // ---- which drafts are kept ----
     if (tid == 0) first_out = n - 1;
     __syncthreads();
-    for (int t = warp; t < n - 1; t += kChoiceWarps) {
-        const int row = r0 + t, x = a.tokens[row + 1];
+    for (int t = warp; t < n; t += kChoiceWarps) {
+        const int row = r0 + t;
+        const float2 *st = a.stats + (size_t)row * a.slices, *sq = a.stats + ((size_t)a.R + min(row + 1, a.R - 1)) * a.slices;
+        const float op = row_offset(st, a.slices);
+        if (t == n - 1) {
+            if (lane == 0 && t < kKept) offset_s[0][t] = op;
+            break;
+        }
+        const int x = a.tokens[row + 1];
+        const float oq = a.draft != nullptr ? row_offset(sq, a.slices) : 0.f;
+        if (lane == 0 && t < kKept) { offset_s[0][t] = op; offset_s[1][t] = oq; }
         bool taken = false;
         if (x >= 0 && x < a.V) {
-            float mp, mq = 0.f;
-            double zp, zq = 1.0, q = 1.0;
-            row_stats(a.stats + (size_t)row * a.slices, a.slices, a.inv, mp, zp);
-            if (a.draft != nullptr) {
-                row_stats(a.stats + ((size_t)a.R + row + 1) * a.slices, a.slices, a.draft_inv, mq, zq);
-                q = exp(((double)tame(bf2f(a.draft[(size_t)(row + 1) * a.draft_stride + x])) - mq) * a.draft_inv) / zq;
-            }
-            const double p = exp(((double)tame(bf2f(a.logits[(size_t)row * a.stride + x])) - mp) * a.inv) / zp;
-            taken = uniform(row, 0) * q < p;     // no probabilities (NaN): not taken
+            const float vp = tame(bf2f(a.logits[(size_t)row * a.stride + x]), a.most);
+            const float vq = a.draft != nullptr ? tame(bf2f(a.draft[(size_t)(row + 1) * a.draft_stride + x]), a.draft_most) : 0.f;
+            const double u = uniform(row, 0);
+            const double q = a.draft == nullptr ? 1.0 : exp2_64(fma((double)vq, (double)a.draft_c, -(double)oq)) / row_sum(sq, a.slices, oq, exp2_64);
+            const double p = exp2_64(fma((double)vp, (double)a.c, -(double)op)) / row_sum(st, a.slices, op, exp2_64);
+            taken = u * q < p;                   // no probabilities (NaN): not taken
         }
         if (!taken && lane == 0) atomicMin(&first_out, t);
     }
@@ -186,64 +245,82 @@ __global__ void __launch_bounds__(kChoiceThreads) verify_choice_kernel(const Ver
     int mode = full ? kAll : a.draft == nullptr ? kWithout : kResidual;
     const int x = full ? -1 : a.tokens[row + 1];
     if (mode == kWithout && (x < 0 || x >= a.V)) mode = kAll;
-    const Row p(a.logits + (size_t)row * a.stride, a.V), q(mode == kResidual ? a.draft + (size_t)(row + 1) * a.draft_stride : a.logits, a.V);
-    float mp, mq = 0.f;
-    double unused;
-    row_stats(a.stats + (size_t)row * a.slices, a.slices, a.inv, mp, unused);
-    if (mode == kResidual) row_stats(a.stats + ((size_t)a.R + row + 1) * a.slices, a.slices, a.draft_inv, mq, unused);
+    const Row p(a.logits + (size_t)row * a.stride, a.V, a.most), q(mode == kResidual ? a.draft + (size_t)(row + 1) * a.draft_stride : a.logits, a.V, a.draft_most);
+    const bool abreast = p.skew == q.skew;       // the two rows' chunks hold the same tokens
+    // any offset that keeps the largest weight near 1 will do: the statistics' one
+    const double op = last < kKept ? offset_s[0][last] : row_offset(a.stats + (size_t)row * a.slices, a.slices);
+    const double oq = mode != kResidual ? 0.f : last < kKept ? offset_s[1][last] : row_offset(a.stats + ((size_t)a.R + row + 1) * a.slices, a.slices);
+    const double goal_u = uniform(row, 1);
     const int chunks = p.chunks(), per = ((chunks + kCluster - 1) / kCluster + 31) / 32 * 32;
     const int lo = min(chunks, rank * per), hi = min(chunks, lo + per), segs = (hi - lo + 31) / 32;
-    double zp = 1.0, zq = 1.0;
-    auto target = [&](float v) -> double { return v > -INFINITY ? exp(((double)v - mp) * a.inv) : 0.0; };
-    auto drafted = [&](int i) -> double {
-        const float v = tame(bf2f(q.p[i]));
-        return v > -INFINITY ? exp(((double)v - mq) * a.draft_inv) : 0.0;
+    double scale_p = 1.0, scale_q = 0.0;
+    auto target = [&](float v) -> double { return exp2_64(fma((double)v, a.c64, -op)); };        // -inf: 0
+    auto drafted = [&](float v) -> double { return exp2_64(fma((double)v, a.draft_c64, -oq)); };
+    auto load_q = [&](int c, float (&v)[8]) {
+        if (abreast) { q.load(c, v); return; }
+        const int i = p.first(c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = i + e >= 0 && i + e < a.V ? tame(bf2f(q.p[i + e]), q.most) : -INFINITY;
     };
     if (mode == kResidual) {
         double sp = 0.0, sq = 0.0;
         for (int c = lo + tid; c < hi; c += kChoiceThreads) {
-            float v[8];
+            float v[8], w[8];
             p.load(c, v);
-            const int i = p.first(c);
+            load_q(c, w);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                sp += target(v[e]);
-                if (i + e >= 0 && i + e < a.V) sq += drafted(i + e);
-            }
+            for (int e = 0; e < 8; ++e) { sp += target(v[e]); sq += drafted(w[e]); }
         }
-        sp = block_sum(sp, warp_s);
-        sq = block_sum(sq, warp_s);
-        if (tid == 0) { share[0] = sp; share[1] = sq; }
+#pragma unroll
+        for (int k = 16; k; k >>= 1) { sp += __shfl_xor_sync(0xffffffffu, sp, k); sq += __shfl_xor_sync(0xffffffffu, sq, k); }
+        if (lane == 0) { part[0][warp] = sp; part[1][warp] = sq; }
+        __syncthreads();
+        if (tid < 2) {
+            double sum = 0.0;
+            for (int w = 0; w < kChoiceWarps; ++w) sum += part[tid][w];
+            share[tid] = sum;
+        }
         cluster.sync();
-        zp = zq = 0.0;
+        double zp = 0.0, zq = 0.0;
+#pragma unroll
         for (int k = 0; k < kCluster; ++k) {
             const double* o = cluster.map_shared_rank(share, k);
             zp += o[0];
             zq += o[1];
         }
-        if (!(zq > 0.0)) zq = INFINITY;          // a drafter without any probability: nothing is taken off
+        scale_p = 1.0 / zp;
+        scale_q = zq > 0.0 ? 1.0 / zq : 0.0;     // a drafter without any probability: nothing is taken off
     }
-    auto weight = [&](float v, int i) -> double {
-        if (i < 0 || i >= a.V || (mode == kWithout && i == x)) return 0.0;
-        const double w = target(v);
-        return mode == kResidual ? fmax(w / zp - drafted(i) / zq, 0.0) : w;
+    auto weights = [&](int c, double (&w)[8]) {  // of chunk c
+        float v[8];
+        p.load(c, v);
+        const int i = p.first(c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = target(v[e]);
+        if (mode == kResidual) {
+            load_q(c, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = fmax(fma(w[e], scale_p, -(drafted(v[e]) * scale_q)), 0.0);
+        } else if (mode == kWithout) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (i + e == x) w[e] = 0.0;
+        }
     };
-    double before = 0.0, total = 0.0;
-    int attempt = 0;
-    for (;; ++attempt) {
+    double before = 0.0, total = 0.0, ends[kCluster];
+    for (int attempt = 0;; ++attempt) {
         for (int s = warp; s < segs; s += kChoiceWarps) {
-            double w = 0.0;
+            double sum = 0.0;
             const int c = lo + s * 32 + lane;
             if (c < hi) {
-                float v[8];
-                p.load(c, v);
-                const int i = p.first(c);
+                double w[8];
+                weights(c, w);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) w += weight(v[e], i + e);
+                for (int e = 0; e < 8; ++e) sum += w[e];
             }
 #pragma unroll
-            for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-            if (lane == 0) seg[s] = w;
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane == 0) seg[s] = sum;
         }
         __syncthreads();
         if (warp == 0) {                         // cumulative weights of the block's segments
@@ -262,26 +339,28 @@ __global__ void __launch_bounds__(kChoiceThreads) verify_choice_kernel(const Ver
         }
         cluster.sync();
         before = total = 0.0;
+#pragma unroll
+        for (int k = 0; k < kCluster; ++k) ends[k] = *cluster.map_shared_rank(share + 2 + attempt, k);
+#pragma unroll
         for (int k = 0; k < kCluster; ++k) {
-            const double w = *cluster.map_shared_rank(share + 2 + attempt, k);
-            if (k < rank) before += w;
-            total += w;
+            if (k < rank) before += ends[k];
+            total += ends[k];
         }
-        // nothing is left where p is nowhere above q but for rounding, or all of it is on the rejected draft: p itself
+        // nothing is left where p is nowhere above q but for rounding, or all of it is on the refused draft: p itself
         if (total > 0.0 || mode == kAll) break;
         mode = kAll;                             // at most once: the second pass ends above
     }
-    // ---- the first token whose cumulative weight is above the target ----
+    // ---- the first token whose cumulative weight is above the goal ----
     if (warp == 0) {
-        const double goal = uniform(row, 1) * total;
+        const double goal = goal_u * total;
         // the block that holds it: the first whose end is above, the last one that has any weight if rounding leaves none
         int owner = -1;
         double sum = 0.0;
+#pragma unroll
         for (int k = 0; k < kCluster; ++k) {
-            const double w = *cluster.map_shared_rank(share + 2 + attempt, k);
             const bool reached = owner >= 0 && goal < sum;
-            sum += w;
-            if (w > 0.0 && !reached) owner = k;
+            sum += ends[k];
+            if (ends[k] > 0.0 && !reached) owner = k;
         }
         if (owner < 0) {
             if (rank == 0 && lane == 0) a.next[seq] = -1;        // a row without any probability
@@ -295,12 +374,11 @@ __global__ void __launch_bounds__(kChoiceThreads) verify_choice_kernel(const Ver
             if (found < 0)                       // rounding: the last segment with any weight
                 for (int s = 0; s < segs; ++s)
                     if (seg[s] > 0.0) found = s;
-            double w[8], own = 0.0;
+            double w[8] = {0, 0, 0, 0, 0, 0, 0, 0}, own = 0.0;
             const int c = lo + found * 32 + lane, i = p.first(c);
-            float v[8];
-            if (c < hi) p.load(c, v);
+            if (c < hi) weights(c, w);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) { w[e] = c < hi ? weight(v[e], i + e) : 0.0; own += w[e]; }
+            for (int e = 0; e < 8; ++e) own += w[e];
             double run = own;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -339,14 +417,15 @@ int tf_verify_rows(const void* logits, size_t row_stride, const void* draft_logi
                    const void* uniforms, int uniforms_f64, int* keep, int* next, void* scratch, size_t scratch_bytes, int rows, int vocab,
                    int n_seqs, double temperature, double draft_temperature, void* stream) {
     if (rows < 1 || rows > 32767 || vocab < 1 || vocab > tf::kMaxVocab || n_seqs < 1 || n_seqs > (1 << 24)) return TF_EINVAL;
-    if (!(temperature > 0.0) || !(draft_temperature > 0.0) || !(temperature < INFINITY) || !(draft_temperature < INFINITY)) return TF_EINVAL;
+    if (!(temperature >= 1e-6) || !(draft_temperature >= 1e-6) || !(temperature <= 1e6) || !(draft_temperature <= 1e6)) return TF_EINVAL;
     if (!logits || !tokens || !seq_start || !uniforms || !keep || !next || row_stride < (size_t)vocab || (draft_logits && draft_stride < (size_t)vocab))
         return TF_EINVAL;
     if (((uintptr_t)logits | (uintptr_t)draft_logits) & 1 || (uintptr_t)uniforms & (uniforms_f64 ? 7 : 3) || (uintptr_t)scratch & 7) return TF_EALIGN;
     if (!scratch || scratch_bytes < tf_verify_scratch_bytes(rows, vocab)) return TF_ESCRATCH;
+    const double c = 1.4426950408889634 / temperature, draft_c = 1.4426950408889634 / draft_temperature, top = 1 << 30;
     tf::VerifyArgs a{static_cast<const __nv_bfloat16*>(logits), static_cast<const __nv_bfloat16*>(draft_logits), row_stride, draft_stride, tokens, seq_start,
                      uniforms, keep, next, static_cast<float2*>(scratch), vocab, rows, n_seqs, (vocab + 7 + tf::kSlice - 1) / tf::kSlice, uniforms_f64,
-                     (float)(1.4426950408889634 / temperature), (float)(1.4426950408889634 / draft_temperature), 1.0 / temperature, 1.0 / draft_temperature};
+                     (float)c, (float)draft_c, (float)(top / c), (float)(top / draft_c), c, draft_c};
     void* args[] = {&a};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (tf::launch_pdl((const void*)tf::verify_stats_kernel, dim3(a.slices, draft_logits ? 2 * rows : rows), dim3(tf::kStatThreads), 0, st, args) !=

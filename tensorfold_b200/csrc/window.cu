@@ -170,23 +170,6 @@ struct Cfg {
     static_assert((kRows - QR) * 128 <= (KS + VS) * TILE_BYTES, "the operand's rows lie inside the block's memory");
 };
 
-// two fp32 values in one register pair: one instruction on both
-__device__ __forceinline__ unsigned long long pair_of(float x, float y) {
-    unsigned long long v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
-    return v;
-}
-__device__ __forceinline__ void split_pair(unsigned long long v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
-__device__ __forceinline__ unsigned long long fma_pair(unsigned long long x, unsigned long long y, unsigned long long z) {
-    unsigned long long v;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(x), "l"(y), "l"(z));
-    return v;
-}
-__device__ __forceinline__ unsigned long long add_pair(unsigned long long x, unsigned long long y) {
-    unsigned long long v;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
-    return v;
-}
 __device__ __forceinline__ float max3(float x, float y, float z) {
     float v;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(x), "f"(y), "f"(z));
