@@ -9,13 +9,13 @@
 //
 // The draw is the first token in vocabulary order whose cumulative weight is above u2 times the total.
 //
-// Two launches. Row statistics: a slice of 8192 logits a block, with y = logit * log2e / T an offset o near its largest y and the sum of
-// 2^(y - o) - bound by the bytes of the logits (128 + 112 rows of 248320: @STATS@). Choice: a cluster of eight blocks per sequence; every block
-// forms the acceptances from the slices' sums (64 bits), then the cluster goes over the one row that is drawn from, twice where
-// a drafter's distribution has to be normalised too - bound by the 64-bit pipe (16 rows of 248320 with a drafter: @CHOICE@, of which two thirds are its ten
-// instructions a weight). An acceptance is one comparison, so 32-bit exponentials (relative error of p and q near 1e-6) decide
-// all but one in a million draws as exact arithmetic would; a draw compares one number with up to a million borders, so its
-// weights and sums are in 64 bits throughout. A NaN logit counts as -inf, +inf as a very
+// Two launches. Row statistics: a slice of 8192 logits a block, an offset o, the largest y = logit * log2e / T, and the sum of 2^(y - o) -
+// bound by the bytes of the logits (128 + 112 rows of 248320: 24 us, 5 TB/s). Choice: a cluster of blocks per sequence; every
+// block forms the acceptances from the slices' sums (64 bits), then the cluster goes over the one row that is drawn from, twice where a
+// drafter's distribution has to be normalised too - bound by the instructions of its 64-bit weights (16 rows of 248320 with a drafter:
+// 42 us; one row without, 11 us, mostly its dependent steps). An acceptance is one comparison, so 32-bit exponentials (relative
+// error of p and q near 1e-6) decide all but one in a million draws as exact arithmetic would; a draw compares one number with
+// up to a million borders, so its weights and sums are in 64 bits throughout (relative error 1e-13). A NaN logit counts as -inf, +inf as a very
 // large one (tame).
 
 #include <cooperative_groups.h>
@@ -28,12 +28,13 @@ namespace cg = cooperative_groups;
 
 constexpr int kStatThreads = 256, kStatChunks = 4;                  // chunks of 8 logits a thread
 constexpr int kSlice = kStatThreads * kStatChunks * 8;              // logits a slice
-constexpr int kChoiceThreads = 1024, kCluster = 8, kChoiceWarps = kChoiceThreads / 32;
+constexpr int kChoiceThreads = 1024, kChoiceWarps = kChoiceThreads / 32;
 constexpr int kKept = 128;                                          // window rows whose offsets are kept between the two steps
 constexpr int kSegment = 256;                                       // logits a warp takes at a time
 constexpr int kMaxVocab = 1 << 20;
 constexpr uint32_t kNone = 0xFF80FF80u;                              // two bf16 -inf
-constexpr int kMaxSegments = kMaxVocab / kCluster / kSegment + 2;
+constexpr int kSpan = 8;                                            // segments a span: the unit that sums are formed in and blocks are given
+constexpr int kMaxSpans = kMaxVocab / (kSegment * kSpan) + 2, kLeastBlocks = 4, kMost = kMaxSpans / kLeastBlocks + 1;   // most: spans a block
 
 struct VerifyArgs {
     const __nv_bfloat16 *logits, *draft;      // rows of V; draft may be null
@@ -60,7 +61,9 @@ struct Row {
     __device__ int first(int c) const { return 8 * c - skew; }
     __device__ uint4 raw(int c) const {          // -inf where there is none
         const int i = first(c);
-        if (i >= 0 && i + 8 <= V) return *reinterpret_cast<const uint4*>(p + i);
+        return i >= 0 && i + 8 <= V ? *reinterpret_cast<const uint4*>(p + i) : edge(i);
+    }
+    __device__ __noinline__ uint4 edge(int i) const {
         uint32_t u[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -69,11 +72,6 @@ struct Row {
             u[e] = lo | hi << 16;
         }
         return make_uint4(u[0], u[1], u[2], u[3]);
-    }
-    __device__ void load(int c, float (&x)[8]) const {
-        unpack8(raw(c), x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = tame(x[e], most);
     }
 };
 
@@ -142,8 +140,8 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
 #pragma unroll 1
         for (int k = 0; k < kStatChunks; ++k) {
             float x[8];
-            if (c0 + k * kStatThreads < chunks) r.load(c0 + k * kStatThreads, x);
-            for (int e = 0; e < 8; ++e) s += c0 + k * kStatThreads < chunks && x[e] > -INFINITY ? fast_exp2(fmaf(x[e], c, -o)) : 0.f;
+            unpack8(c0 + k * kStatThreads < chunks ? r.raw(c0 + k * kStatThreads) : make_uint4(kNone, kNone, kNone, kNone), x);
+            for (int e = 0; e < 8; ++e) s += fast_exp2(fmaf(tame(x[e], r.most), c, -o));
         }
         s = warp_sum(s);
         __syncthreads();
@@ -155,24 +153,37 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
     if (tid == 0) a.stats[(size_t)blockIdx.y * a.slices + blockIdx.x] = make_float2(o, s);
 }
 
-// 2^t for t < 1000 in 64 bits: t = n / 64 + r, a table of 2^(j/64), and the series of 2^r = e^(r ln 2) to the fifth power (|r| <= 1/128: the
-// next term is 4e-17). Zero below 2^-1000.
-struct Exp2 {
+// A weight 2^(logit c - offset) in 64 bits, in the two factors of which the second is a table's: t = 16 (logit c - offset) = n + r, a table of
+// 2^(j/16) times a factor of the row's own (128 bytes: no two entries share a bank; the high words less j << 16, so that adding n << 16 sets the
+// exponent), and the series of 2^(r/16) to the fifth power (the next term is 1.5e-13 at |r| = 1/2). Ten operations of the 64-bit pipe
+// with the product and eight others: the kernel is bound by how many instructions a weight takes. Weights end at 2^-900, which stands for 0 (NaN and
+// -inf too): sums and weights up to kZero are none.
+constexpr int kTable = 16;
+constexpr double kZero = 1e-240;
+__device__ __forceinline__ double table_entry(double value, int j) { return __hiloint2double(__double2hiint(value) - (j << 16), __double2loint(value)); }
+struct Weight {
+    double slope, shift;                         // 16 c, 16 offset
+    float least, most;                           // logit of 2^-900, of the largest that counts
     const double* table;                         // shared memory
-    __device__ double operator()(double t) const {
-        constexpr double l = 0.69314718055994530942;
-        const double shifter = 6755399441055744.0;                     // 1.5 * 2^52: adding it leaves the nearest integer in the low word
-        const double big = fma(t, 64.0, shifter);
+    // (a row of nothing has no offset: any will do)
+    __device__ Weight(double c, float offset, float most_, const double* table_)
+        : slope(kTable * c), shift(offset > -INFINITY ? kTable * (double)offset : 0.0), least((float)((shift / kTable - 900.0) / c)), most(most_), table(table_) {}
+    __device__ void operator()(float v, double& series, double& factor) const {
+        constexpr double l = 0.69314718055994530942 / kTable, shifter = 6755399441055744.0;   // 1.5 * 2^52: adding it leaves the nearest integer in the low word
+        const double t = fma((double)fminf(fmaxf(v, least), most), slope, -shift), big = t + shifter, r = t - (big - shifter);
         const int n = __double2loint(big);
-        const double r = fma(big - shifter, -1.0 / 64.0, t);
         double y = fma(r, l * l * l * l * l / 120, l * l * l * l / 24);
         y = fma(r, y, l * l * l / 6);
         y = fma(r, y, l * l / 2);
         y = fma(r, y, l);
-        y = fma(r, y, 1.0);
-        const double p = table[n & 63];
-        const double scaled = __hiloint2double(__double2hiint(p) + ((n >> 6) << 20), __double2loint(p));
-        return t > -1000.0 ? y * scaled : 0.0;
+        series = fma(r, y, 1.0);
+        const double p = table[n & (kTable - 1)];
+        factor = __hiloint2double(__double2hiint(p) + (n << 16), __double2loint(p));
+    }
+    __device__ double operator()(float v) const {
+        double y, f;
+        (*this)(v, y, f);
+        return y * f;
     }
 };
 
@@ -182,10 +193,10 @@ __device__ __forceinline__ float row_offset(const float2* st, int slices) {
     for (int i = threadIdx.x & 31; i < slices; i += 32) o = fmaxf(o, st[i].x);
     return warp_max(o);
 }
-__device__ __forceinline__ double row_sum(const float2* st, int slices, float o, const Exp2& exp2_64) {
+__device__ __forceinline__ double row_sum(const float2* st, int slices, float o, const double* table) {
+    const Weight w(1.0, o, 3e9f, table);
     double z = 0.0;
-    for (int i = threadIdx.x & 31; i < slices; i += 32)
-        if (st[i].x > -INFINITY) z += st[i].y * exp2_64((double)st[i].x - o);
+    for (int i = threadIdx.x & 31; i < slices; i += 32) z += st[i].y * w(st[i].x);           // a slice of nothing has the sum 0
 #pragma unroll
     for (int k = 16; k; k >>= 1) z += __shfl_xor_sync(0xffffffffu, z, k);
     return z;
@@ -194,21 +205,21 @@ __device__ __forceinline__ double row_sum(const float2* st, int slices, float o,
 enum Weights { kAll, kWithout, kResidual };     // p; p without the draft; max(p - q, 0)
 
 __global__ void __launch_bounds__(kChoiceThreads, 1) verify_choice_kernel(const VerifyArgs a) {
-    __shared__ double table[64], part[2][kChoiceWarps], seg[kMaxSegments], cum[kMaxSegments], share[4];
+    // sums of the block's spans: [0] p, [1] q, then the weights of the first and the second attempt; of its segments; of every block's spans
+    __shared__ double table[kTable], table_p[kTable], table_q[kTable], span_s[4][kMost], seg[2 * kMost * kSpan], all_s[kMaxSpans];
     __shared__ float offset_s[2][kKept];         // target's and drafter's, of the window's first rows
     __shared__ int first_out;
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (tid < 64) table[tid] = exp2(tid / 64.0);
+    if (tid < kTable) table[tid] = table_p[tid] = table_q[tid] = table_entry(exp2(tid / (double)kTable), tid);
     pdl_launch_dependents();
     pdl_wait();
-    const int seq = blockIdx.x / kCluster, rank = blockIdx.x % kCluster;
+    const int blocks = cluster.num_blocks(), rank = cluster.block_rank(), seq = blockIdx.x / blocks;
     const int r0 = a.seq_start[seq], n = a.seq_start[seq + 1] - r0;
     if (n < 1) {                                 // a sequence without rows: the whole cluster leaves
         if (rank == 0 && tid == 0) { a.keep[seq] = 0; a.next[seq] = -1; }
         return;
     }
-    const Exp2 exp2_64{table};
     auto uniform = [&](int row, int i) -> double {
         return a.u64 ? static_cast<const double*>(a.uniforms)[2 * (size_t)row + i] : (double)static_cast<const float*>(a.uniforms)[2 * (size_t)row + i];
     };
@@ -231,8 +242,8 @@ __global__ void __launch_bounds__(kChoiceThreads, 1) verify_choice_kernel(const 
             const float vp = tame(bf2f(a.logits[(size_t)row * a.stride + x]), a.most);
             const float vq = a.draft != nullptr ? tame(bf2f(a.draft[(size_t)(row + 1) * a.draft_stride + x]), a.draft_most) : 0.f;
             const double u = uniform(row, 0);
-            const double q = a.draft == nullptr ? 1.0 : exp2_64(fma((double)vq, (double)a.draft_c, -(double)oq)) / row_sum(sq, a.slices, oq, exp2_64);
-            const double p = exp2_64(fma((double)vp, (double)a.c, -(double)op)) / row_sum(st, a.slices, op, exp2_64);
+            const double q = a.draft == nullptr ? 1.0 : Weight(a.draft_c, oq, a.draft_most, table)(vq) / row_sum(sq, a.slices, oq, table);
+            const double p = vp > -INFINITY ? Weight(a.c, op, a.most, table)(vp) / row_sum(st, a.slices, op, table) : 0.0;
             taken = u * q < p;                   // no probabilities (NaN): not taken
         }
         if (!taken && lane == 0) atomicMin(&first_out, t);
@@ -248,71 +259,92 @@ __global__ void __launch_bounds__(kChoiceThreads, 1) verify_choice_kernel(const 
     const Row p(a.logits + (size_t)row * a.stride, a.V, a.most), q(mode == kResidual ? a.draft + (size_t)(row + 1) * a.draft_stride : a.logits, a.V, a.draft_most);
     const bool abreast = p.skew == q.skew;       // the two rows' chunks hold the same tokens
     // any offset that keeps the largest weight near 1 will do: the statistics' one
-    const double op = last < kKept ? offset_s[0][last] : row_offset(a.stats + (size_t)row * a.slices, a.slices);
-    const double oq = mode != kResidual ? 0.f : last < kKept ? offset_s[1][last] : row_offset(a.stats + ((size_t)a.R + row + 1) * a.slices, a.slices);
+    const float op = last < kKept ? offset_s[0][last] : row_offset(a.stats + (size_t)row * a.slices, a.slices);
+    const float oq = mode != kResidual ? 0.f : last < kKept ? offset_s[1][last] : row_offset(a.stats + ((size_t)a.R + row + 1) * a.slices, a.slices);
     const double goal_u = uniform(row, 1);
-    const int chunks = p.chunks(), per = ((chunks + kCluster - 1) / kCluster + 31) / 32 * 32;
-    const int lo = min(chunks, rank * per), hi = min(chunks, lo + per), segs = (hi - lo + 31) / 32;
-    double scale_p = 1.0, scale_q = 0.0;
-    auto target = [&](float v) -> double { return exp2_64(fma((double)v, a.c64, -op)); };        // -inf: 0
-    auto drafted = [&](float v) -> double { return exp2_64(fma((double)v, a.draft_c64, -oq)); };
-    auto load_q = [&](int c, float (&v)[8]) {
-        if (abreast) { q.load(c, v); return; }
-        const int i = p.first(c);
+    // the row in spans of 512 chunks, dealt out in runs; sums are formed by span and then over the spans in order, so that they do not depend
+    // on how many blocks the cluster has
+    const int chunks = p.chunks(), spans = (chunks + kSpan * 32 - 1) / (kSpan * 32), least = spans / blocks, more = spans - least * blocks;
+    const int first = rank * least + min(rank, more), mine = least + (rank < more), lo = first * kSpan * 32, segs = mine * kSpan;
+    // the block that holds span `tid`, and where
+    const int in_more = more * (least + 1), holder = tid < in_more ? tid / (least + 1) : more + (tid - in_more) / max(least, 1);
+    const int held_at = tid - holder * least - min(holder, more);
+    const Weight target(a.c64, op, a.most, table_p), drafted(a.draft_c64, oq, a.draft_most, table_q);
+    auto load_q = [&](int c, float (&v)[8]) { unpack8(abreast ? q.raw(c) : q.edge(p.first(c)), v); };
+    // the sum over all spans of the cluster, `which` of the span sums, in order; all_s keeps them. The whole block; the clusters' span sums are
+    // complete (a cluster barrier lies before).
+    auto gather = [&](int which) -> double {
+        static_assert(kMaxSpans <= kChoiceThreads, "a thread a span");
+        __syncthreads();                         // all_s is no longer read
+        if (tid < spans) all_s[tid] = cluster.map_shared_rank(&span_s[which][0], holder)[held_at];
+        __syncthreads();
+        double sum = 0.0;
+        for (int i = lane; i < spans; i += 32) sum += all_s[i];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = i + e >= 0 && i + e < a.V ? tame(bf2f(q.p[i + e]), q.most) : -INFINITY;
+        for (int k = 16; k; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+        return sum;
     };
     if (mode == kResidual) {
-        double sp = 0.0, sq = 0.0;
-        for (int c = lo + tid; c < hi; c += kChoiceThreads) {
-            float v[8], w[8];
-            p.load(c, v);
-            load_q(c, w);
+        // a warp a segment of 256 tokens; p and q of the span's segments are added by its sixteen warps' lanes below
+        for (int s = warp; s < segs; s += kChoiceWarps) {
+            double sp = 0.0, sq = 0.0;
+            const int c = lo + s * 32 + lane;
+            if (c < chunks) {
+                float v[8], w[8];
+                unpack8(p.raw(c), v);
+                load_q(c, w);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) { sp += target(v[e]); sq += drafted(w[e]); }
+                for (int e = 0; e < 8; ++e) { sp += target(v[e]); sq += drafted(w[e]); }
+            }
+#pragma unroll
+            for (int k = 16; k; k >>= 1) { sp += __shfl_xor_sync(0xffffffffu, sp, k); sq += __shfl_xor_sync(0xffffffffu, sq, k); }
+            if (lane == 0) { seg[s] = sp; seg[segs + s] = sq; }
         }
-#pragma unroll
-        for (int k = 16; k; k >>= 1) { sp += __shfl_xor_sync(0xffffffffu, sp, k); sq += __shfl_xor_sync(0xffffffffu, sq, k); }
-        if (lane == 0) { part[0][warp] = sp; part[1][warp] = sq; }
         __syncthreads();
-        if (tid < 2) {
+        for (int i = tid; i < 2 * mine; i += kChoiceThreads) {
+            const double* from = seg + (i < mine ? 0 : segs) + (i < mine ? i : i - mine) * kSpan;
             double sum = 0.0;
-            for (int w = 0; w < kChoiceWarps; ++w) sum += part[tid][w];
-            share[tid] = sum;
+#pragma unroll
+            for (int k = 0; k < kSpan; ++k) sum += from[k];
+            span_s[i < mine ? 0 : 1][i < mine ? i : i - mine] = sum;
         }
         cluster.sync();
-        double zp = 0.0, zq = 0.0;
-#pragma unroll
-        for (int k = 0; k < kCluster; ++k) {
-            const double* o = cluster.map_shared_rank(share, k);
-            zp += o[0];
-            zq += o[1];
+        const double zp = gather(0), zq = gather(1);
+        // the normalisers go into the tables; a drafter without any probability takes nothing off (2^-900 a token)
+        if (tid < kTable) {
+            const double whole = exp2(tid / (double)kTable);
+            table_p[tid] = table_entry(zp > kZero ? whole / zp : whole, tid);
+            table_q[tid] = table_entry(zq > kZero ? whole / zq : whole, tid);
         }
-        scale_p = 1.0 / zp;
-        scale_q = zq > 0.0 ? 1.0 / zq : 0.0;     // a drafter without any probability: nothing is taken off
+        __syncthreads();
     }
     auto weights = [&](int c, double (&w)[8]) {  // of chunk c
         float v[8];
-        p.load(c, v);
+        unpack8(p.raw(c), v);
         const int i = p.first(c);
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = target(v[e]);
         if (mode == kResidual) {
             load_q(c, v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = fmax(fma(w[e], scale_p, -(drafted(v[e]) * scale_q)), 0.0);
+            for (int e = 0; e < 8; ++e) {
+                double y, f;
+                drafted(v[e], y, f);
+                const double rest = fma(-y, f, w[e]);
+                w[e] = __double2hiint(rest) < 0 ? 0.0 : rest;
+            }
         } else if (mode == kWithout) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 if (i + e == x) w[e] = 0.0;
         }
     };
-    double before = 0.0, total = 0.0, ends[kCluster];
+    double total;
     for (int attempt = 0;; ++attempt) {
         for (int s = warp; s < segs; s += kChoiceWarps) {
             double sum = 0.0;
             const int c = lo + s * 32 + lane;
-            if (c < hi) {
+            if (c < chunks) {
                 double w[8];
                 weights(c, w);
 #pragma unroll
@@ -323,60 +355,56 @@ __global__ void __launch_bounds__(kChoiceThreads, 1) verify_choice_kernel(const 
             if (lane == 0) seg[s] = sum;
         }
         __syncthreads();
-        if (warp == 0) {                         // cumulative weights of the block's segments
-            double base = 0.0;
-            for (int s0 = 0; s0 < segs; s0 += 32) {
-                double w = s0 + lane < segs ? seg[s0 + lane] : 0.0;
+        for (int i = tid; i < mine; i += kChoiceThreads) {
+            double sum = 0.0;
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double y = __shfl_up_sync(0xffffffffu, w, o);
-                    if (lane >= o) w += y;
-                }
-                if (s0 + lane < segs) cum[s0 + lane] = base + w;
-                base += __shfl_sync(0xffffffffu, w, 31);
-            }
-            if (lane == 0) share[2 + attempt] = base;
+            for (int k = 0; k < kSpan; ++k) sum += seg[i * kSpan + k];
+            span_s[2 + attempt][i] = sum;
         }
         cluster.sync();
-        before = total = 0.0;
-#pragma unroll
-        for (int k = 0; k < kCluster; ++k) ends[k] = *cluster.map_shared_rank(share + 2 + attempt, k);
-#pragma unroll
-        for (int k = 0; k < kCluster; ++k) {
-            if (k < rank) before += ends[k];
-            total += ends[k];
-        }
+        total = gather(2 + attempt);
         // nothing is left where p is nowhere above q but for rounding, or all of it is on the refused draft: p itself
-        if (total > 0.0 || mode == kAll) break;
+        if (total > kZero || mode == kAll) break;
         mode = kAll;                             // at most once: the second pass ends above
     }
     // ---- the first token whose cumulative weight is above the goal ----
     if (warp == 0) {
         const double goal = goal_u * total;
-        // the block that holds it: the first whose end is above, the last one that has any weight if rounding leaves none
-        int owner = -1;
-        double sum = 0.0;
+        // a warp's search in `count` weights: the first whose cumulative weight is above `at`, or the last with any if rounding leaves none; `at`
+        // becomes what is left of it there. -1: no weight at all
+        auto search = [&](const double* w, int count, double& at) -> int {
+            double base = 0.0, start_of_last = 0.0;
+            int last_with = -1;
+            for (int i0 = 0; i0 < count; i0 += 32) {
+                const double v = i0 + lane < count ? w[i0 + lane] : 0.0;
+                double run = v;
 #pragma unroll
-        for (int k = 0; k < kCluster; ++k) {
-            const bool reached = owner >= 0 && goal < sum;
-            sum += ends[k];
-            if (ends[k] > 0.0 && !reached) owner = k;
-        }
-        if (owner < 0) {
-            if (rank == 0 && lane == 0) a.next[seq] = -1;        // a row without any probability
-        } else if (owner == rank) {
-            const double at = goal - before;
-            int found = -1;
-            for (int s0 = 0; s0 < segs && found < 0; s0 += 32) {
-                const unsigned m = __ballot_sync(0xffffffffu, s0 + lane < segs && seg[s0 + lane] > 0.0 && cum[s0 + lane] > at);
-                if (m) found = s0 + __ffs(m) - 1;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double y = __shfl_up_sync(0xffffffffu, run, o);
+                    if (lane >= o) run += y;
+                }
+                run += base;
+                const unsigned above = __ballot_sync(0xffffffffu, v > kZero && run > at), any = __ballot_sync(0xffffffffu, v > kZero);
+                const int who = above ? __ffs(above) - 1 : 31 - __clz(any);
+                if (any) {
+                    last_with = i0 + who;
+                    start_of_last = __shfl_sync(0xffffffffu, run - v, who);
+                }
+                if (above) break;
+                base = __shfl_sync(0xffffffffu, run, 31);
             }
-            if (found < 0)                       // rounding: the last segment with any weight
-                for (int s = 0; s < segs; ++s)
-                    if (seg[s] > 0.0) found = s;
+            at -= start_of_last;
+            return last_with;
+        };
+        double at = goal;
+        const int span = search(all_s, spans, at);
+        if (span < 0) {
+            if (rank == 0 && lane == 0) a.next[seq] = -1;        // a row without any probability
+        } else if (span >= first && span < first + mine) {
+            const int found = (span - first) * kSpan + search(seg + (span - first) * kSpan, kSpan, at);
             double w[8] = {0, 0, 0, 0, 0, 0, 0, 0}, own = 0.0;
             const int c = lo + found * 32 + lane, i = p.first(c);
-            if (c < hi) weights(c, w);
+            if (c < chunks) weights(c, w);
 #pragma unroll
             for (int e = 0; e < 8; ++e) own += w[e];
             double run = own;
@@ -385,12 +413,12 @@ __global__ void __launch_bounds__(kChoiceThreads, 1) verify_choice_kernel(const 
                 const double y = __shfl_up_sync(0xffffffffu, run, o);
                 if (lane >= o) run += y;
             }
-            run += (found > 0 ? cum[found - 1] : 0.0) - own;
+            run -= own;
             int hit = -1, positive = -1;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 run += w[e];
-                if (w[e] > 0.0) {
+                if (w[e] > kZero) {
                     positive = i + e;
                     if (hit < 0 && run > at) hit = i + e;
                 }
@@ -401,6 +429,35 @@ __global__ void __launch_bounds__(kChoiceThreads, 1) verify_choice_kernel(const 
         }
     }
     cluster.sync();                              // nobody leaves while another block may read its sums
+}
+
+// Blocks a sequence: as many as still let all sequences' clusters run at the same time, which the GPU is asked once (of 148 SMs, for
+// instance, 7 clusters of 16, 15 of 8, 22 of 6 fit: 16 sequences as clusters of 8 took two rounds, 53 us against 50 of 6 at the time). Four where even those do not.
+int cluster_for(int n_seqs) {
+    constexpr int kSizes[] = {16, 8, 6, kLeastBlocks};
+    static int fits[64][4];                      // per device; 0: not asked yet
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return 0; }
+    if (fits[dev][3] == 0) {
+        if (cudaFuncSetAttribute(verify_choice_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) { cudaGetLastError(); return 0; }
+        for (int i = 0; i < 4; ++i) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(kSizes[i]);
+            cfg.blockDim = dim3(kChoiceThreads);
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = kSizes[i];
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            int n = 0;
+            if (cudaOccupancyMaxActiveClusters(&n, verify_choice_kernel, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
+            fits[dev][i] = n < 1 ? -1 : n;
+        }
+    }
+    for (int i = 0; i < 3; ++i)
+        if (fits[dev][i] >= n_seqs) return kSizes[i];
+    return fits[dev][3] > 0 ? kLeastBlocks : 0;
 }
 
 }  // namespace
@@ -430,13 +487,15 @@ int tf_verify_rows(const void* logits, size_t row_stride, const void* draft_logi
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (tf::launch_pdl((const void*)tf::verify_stats_kernel, dim3(a.slices, draft_logits ? 2 * rows : rows), dim3(tf::kStatThreads), 0, st, args) !=
         cudaSuccess) { cudaGetLastError(); return TF_ECUDA; }
+    const int blocks = tf::cluster_for(n_seqs);
+    if (blocks < 1) return TF_ECUDA;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(n_seqs * tf::kCluster);
+    cfg.gridDim = dim3(n_seqs * blocks);
     cfg.blockDim = dim3(tf::kChoiceThreads);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = tf::kCluster;
+    attr[0].val.clusterDim.x = blocks;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
