@@ -95,14 +95,20 @@ __global__ void __launch_bounds__(kMassThreads, 1) mass_kernel(const __grid_cons
     if (warp == kMassLoad) {
         const int* pt = a.page_table + (size_t)seq * a.max_pages;
         Ring ring(KS, 1);
-        for (int t = first; t < last; ++t) {
-            // eight pages, a lane each; one behind the last key or that is none (reported) is copied from page 0 and not used
-            int page = 0;
+        // a tile's eight pages, a lane each, looked up a tile ahead; one behind the last key or that is none (reported) is copied from
+        // page 0 and not used
+        auto number = [&](int t) -> int {
             const int j = t * kMassKeys + lane * kPage;
-            if (lane < 8 && j < keys) {
-                page = pt[j / kPage];
-                if (page < 0 || page >= a.num_pages) { report(a.status, TF_EINVAL); page = 0; }
-            }
+            if (lane >= 8 || t >= last || j >= keys) return 0;
+            const int page = pt[j / kPage];
+            if (page >= 0 && page < a.num_pages) return page;
+            report(a.status, TF_EINVAL);
+            return 0;
+        };
+        int next = number(first);
+        for (int t = first; t < last; ++t) {
+            const int page = next;
+            next = number(t + 1);
             wait(k_empty(ring.i), ring.phase);
             if (lane == 0) mbar_arrive_expect_tx(k_full(ring.i), C::TILE_BYTES);
             __syncwarp();
@@ -155,10 +161,19 @@ __global__ void __launch_bounds__(kMassThreads, 1) mass_kernel(const __grid_cons
         auto stage = [&](int c) {            // rows c * 128 ..: into shared memory, with their log-sum-exps
             const int q0 = c * kMassRows, count = min(kMassRows, rows - q0);
             const size_t row0 = (size_t)layer * a.R + r0;
-            for (int e = tid; e < count * CPR; e += kMassSum * 32) {
-                const int r = e / CPR, x = e % CPR, t = (q0 + r) / G;
-                const uint4 v = *reinterpret_cast<const uint4*>(a.q + ((row0 + t) * a.H + kvh * G + q0 + r - t * G) * D + x * 8);
-                *reinterpret_cast<uint4*>(q_s + (x >> 3) * C::Q_SLAB + r * 128 + (((x ^ r) & 7) << 4)) = v;
+            constexpr int B = 8, STEP = kMassSum * 32;       // loads in flight a thread
+            for (int e0 = tid; e0 < count * CPR; e0 += B * STEP) {
+                uint4 v[B];
+#pragma unroll
+                for (int k = 0; k < B; ++k) {
+                    const int e = min(e0 + k * STEP, count * CPR - 1), r = e / CPR, x = e % CPR, t = (q0 + r) / G;
+                    v[k] = *reinterpret_cast<const uint4*>(a.q + ((row0 + t) * a.H + kvh * G + q0 + r - t * G) * D + x * 8);
+                }
+#pragma unroll
+                for (int k = 0; k < B; ++k) {
+                    const int e = e0 + k * STEP, r = e / CPR, x = e % CPR;
+                    if (e < count * CPR) *reinterpret_cast<uint4*>(q_s + (x >> 3) * C::Q_SLAB + r * 128 + (((x ^ r) & 7) << 4)) = v[k];
+                }
             }
             if (tid < count) {
                 const int t = (q0 + tid) / G;
@@ -262,70 +277,124 @@ __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, u
     return before + x - v;
 }
 
+// Bound by its chain of dependent steps (4224 slots: 12.9 us with 64 of them on the GPU): the page numbers, then weights and positions, a
+// quarter page a thread; three histogram passes over the keys in shared memory, in which the slots that stay anyway take no part; one
+// pass that counts, one that writes.
 template <bool STAGED>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictArgs a) {
     extern __shared__ uint32_t keys_s[];
     __shared__ unsigned hist[kBins];
     __shared__ unsigned long long warp_s[kSelThreads / 32];
-    __shared__ unsigned digit_s, above_s;
+    __shared__ unsigned digit_s, above_s, safe_s;
     pdl_launch_dependents();
-    pdl_wait();
     const int kvh = blockIdx.x, seq = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x;
     const size_t item = ((size_t)layer * a.S + seq) * a.HK + kvh;
-    const int L = a.seq_lens[seq], n = min(L, min(a.max_context, a.max_pages * kPage));
+    for (int b = tid; b < kBins; b += kSelThreads) hist[b] = 0;
+    if (tid == 0) safe_s = 0;
+    pdl_wait();
+    const int L = a.seq_lens[seq], n = min(L, min(a.max_context, a.max_pages * kPage)), safe_from = a.next_pos[seq] - a.recent;
     if (L > n && tid == 0) report(a.status, TF_EINVAL);
     if (n <= a.budget) {
         if (tid == 0) a.moved[item] = 0;
         return;
     }
     const int* pt = a.page_table + (size_t)seq * a.max_pages;
-    const int safe_from = a.next_pos[seq] - a.recent;
+    constexpr uint32_t kSafe = 0xFFFFFFFFu;
     // a slot's rank: protected first, then by mass; NaN counts as -inf
-    auto rank_of = [&](int j) -> uint32_t {
-        const int page = pt[j / kPage];
-        if (page < 0 || page >= a.num_pages) { report(a.status, TF_EINVAL); return 0u; }
-        const size_t cell = (((size_t)layer * a.num_pages + page) * a.HK + kvh) * kPage + j % kPage;
-        const int p = a.pos[cell];
-        if (p < a.sinks || p >= safe_from) return 0xFFFFFFFFu;
-        const float m = a.mass[cell] + 0.f;            // -0 ranks as 0
-        if (m != m) return 0x007FFFFFu;                // the rank of -inf
+    auto rank_of = [&](float m, int p) -> uint32_t {
+        if (p < a.sinks || p >= safe_from) return kSafe;
+        m += 0.f;                                      // -0 ranks as 0
         const uint32_t u = __float_as_uint(m);
-        return u & 0x80000000u ? ~u : u | 0x80000000u;
+        return m != m ? 0x007FFFFFu : u & 0x80000000u ? ~u : u | 0x80000000u;
     };
-    auto key = [&](int j) -> uint32_t { return STAGED ? keys_s[j] : rank_of(j); };
-    if (STAGED)
-        for (int j = tid; j < n; j += kSelThreads) keys_s[j] = rank_of(j);
-
-    // the budget-th largest key, 11 + 11 + 10 bits at a time
-    uint32_t prefix = 0, need = a.budget;
-    for (int pass = 0; pass < 3; ++pass) {
-        const int bits = pass == 2 ? 10 : 11, shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-        __syncthreads();
-        for (int b = tid; b < kBins; b += kSelThreads) hist[b] = 0;
-        __syncthreads();
-        for (int j = tid; j < n; j += kSelThreads) {
-            const uint32_t k = key(j);
-            if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+    auto cell_of = [&](int j, int page) -> size_t { return (((size_t)layer * a.num_pages + page) * a.HK + kvh) * kPage + j % kPage; };
+    auto page_of = [&](int j) -> int {
+        const int page = pt[j / kPage];
+        if (page < 0 || page >= a.num_pages) { report(a.status, TF_EINVAL); return -1; }
+        return page;
+    };
+    auto key = [&](int j) -> uint32_t {
+        if (STAGED) return keys_s[j];
+        const int page = page_of(j);
+        return page < 0 ? 0u : rank_of(a.mass[cell_of(j, page)], a.pos[cell_of(j, page)]);
+    };
+    __syncthreads();
+    unsigned safe = 0;
+    if (STAGED) {
+        // four slots a thread, two such quads in flight; the first histogram on the way
+        for (int q0 = tid; q0 * 4 < n; q0 += 2 * kSelThreads) {
+            int page[2];
+            float4 m[2];
+            int4 p[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) page[k] = (q0 + k * kSelThreads) * 4 < n ? page_of((q0 + k * kSelThreads) * 4) : -1;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const size_t cell = cell_of((q0 + k * kSelThreads) * 4, max(page[k], 0));
+                m[k] = page[k] < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *reinterpret_cast<const float4*>(a.mass + cell);
+                p[k] = page[k] < 0 ? make_int4(0, 0, 0, 0) : *reinterpret_cast<const int4*>(a.pos + cell);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int j = (q0 + k * kSelThreads) * 4;
+                const float mk[4] = {m[k].x, m[k].y, m[k].z, m[k].w};
+                const int pk[4] = {p[k].x, p[k].y, p[k].z, p[k].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (j + e >= n) continue;
+                    const uint32_t r = page[k] < 0 ? 0u : rank_of(mk[e], pk[e]);
+                    keys_s[j + e] = r;
+                    if (r == kSafe) ++safe;
+                    else atomicAdd(&hist[r >> 21], 1u);
+                }
+            }
         }
-        __syncthreads();
-        // thread i holds bins 2047 - 2i and 2046 - 2i: prefix sums from the largest digit down
-        const unsigned c0 = hist[kBins - 1 - 2 * tid], c1 = hist[kBins - 2 - 2 * tid];
-        unsigned long long total;
-        const unsigned before = (unsigned)block_scan(c0 + c1, warp_s, total);
-        if (before < need && before + c0 >= need) { digit_s = kBins - 1 - 2 * tid; above_s = before; }
-        else if (before + c0 < need && before + c0 + c1 >= need) { digit_s = kBins - 2 - 2 * tid; above_s = before + c0; }
-        __syncthreads();
-        prefix = prefix << bits | digit_s;
-        need -= above_s;
+    } else {
+        for (int j = tid; j < n; j += kSelThreads) {
+            const uint32_t r = key(j);
+            if (r == kSafe) ++safe;
+            else atomicAdd(&hist[r >> 21], 1u);
+        }
+    }
+    safe = __reduce_add_sync(0xffffffffu, safe);
+    if ((tid & 31) == 0 && safe) atomicAdd(&safe_s, safe);
+    __syncthreads();
+    // the smallest key that stays, 11 + 11 + 10 bits at a time: the need-th largest of those that are not protected. More protected slots than
+    // the budget holds (positions that are none): the first of them stay
+    uint32_t prefix = kSafe, need = a.budget;
+    if (safe_s < need) {
+        need -= safe_s;
+        prefix = 0;
+        for (int pass = 0; pass < 3; ++pass) {
+            const int bits = pass == 2 ? 10 : 11, shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+            if (pass > 0) {
+                for (int b = tid; b < kBins; b += kSelThreads) hist[b] = 0;
+                __syncthreads();
+                for (int j = tid; j < n; j += kSelThreads) {
+                    const uint32_t k = key(j);
+                    if ((k >> (shift + bits)) == prefix && k != kSafe) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+                }
+                __syncthreads();
+            }
+            // thread i holds bins 2047 - 2i and 2046 - 2i: prefix sums from the largest digit down
+            const unsigned c0 = hist[kBins - 1 - 2 * tid], c1 = hist[kBins - 2 - 2 * tid];
+            unsigned long long total;
+            const unsigned before = (unsigned)block_scan(c0 + c1, warp_s, total);
+            if (before < need && before + c0 >= need) { digit_s = kBins - 1 - 2 * tid; above_s = before; }
+            else if (before + c0 < need && before + c0 + c1 >= need) { digit_s = kBins - 2 - 2 * tid; above_s = before + c0; }
+            __syncthreads();
+            prefix = prefix << bits | digit_s;
+            need -= above_s;
+        }
     }
     // kept: every key above `prefix` and the first `need` slots of that key. Each thread takes a run of slots (an odd number of
     // words: no bank conflicts)
     const int per = ((n + kSelThreads - 1) / kSelThreads) | 1, lo = min(n, tid * per), hi = min(n, lo + per);
-    unsigned long long equal = 0, total;
-    for (int j = lo; j < hi; ++j) equal += key(j) == prefix;
-    const unsigned eq0 = (unsigned)block_scan(equal, warp_s, total);
+    unsigned long long counts = 0, total;
+    for (int j = lo; j < hi; ++j) counts += key(j) == prefix;
+    const unsigned eq0 = (unsigned)block_scan(counts, warp_s, total);
     unsigned eq = eq0;
-    unsigned long long counts = 0;               // holes below the budget | kept slots above it
+    counts = 0;                                  // holes below the budget | kept slots above it
     for (int j = lo; j < hi; ++j) {
         const uint32_t k = key(j);
         const bool kept = k > prefix || (k == prefix && eq++ < need);
@@ -362,20 +431,39 @@ __global__ void __launch_bounds__(kMoveWarps * 32) evict_move_kernel(const Evict
         ok = ok && page >= 0 && page < a.num_pages;
         return (((size_t)layer * a.num_pages + page) * a.HK + kvh) * kPage + j % kPage;
     };
-    for (int i = blockIdx.x * kMoveWarps + warp; i < count; i += gridDim.x * kMoveWarps) {
-        bool ok = true;
-        const size_t to = cell(holes[i], ok), from = cell(fills[i], ok);
-        if (!ok) continue;
-        if (D == 256) {
-            const uint4 k = reinterpret_cast<const uint4*>(a.k_pages + from * D)[lane], v = reinterpret_cast<const uint4*>(a.v_pages + from * D)[lane];
-            reinterpret_cast<uint4*>(a.k_pages + to * D)[lane] = k;
-            reinterpret_cast<uint4*>(a.v_pages + to * D)[lane] = v;
-        } else {
-            __nv_bfloat16* base = lane < 16 ? a.k_pages : a.v_pages;
-            const uint4 x = reinterpret_cast<const uint4*>(base + from * D)[lane & 15];
-            reinterpret_cast<uint4*>(base + to * D)[lane & 15] = x;
+    // four slots a warp at a time: their places are looked up by four lanes, then eight rows (four of K, four of V) are on the way together
+    constexpr int B = 4;
+    for (int i0 = (blockIdx.x * kMoveWarps + warp) * B; i0 < count; i0 += gridDim.x * kMoveWarps * B) {
+        bool ok = lane < B && i0 + lane < count;
+        long long to = 0, from = 0;
+        if (ok) {
+            to = cell(holes[i0 + lane], ok);
+            from = cell(fills[i0 + lane], ok);
         }
-        if (lane == 0) { a.mass[to] = a.mass[from]; a.pos[to] = a.pos[from]; }
+        const float m = ok ? a.mass[from] : 0.f;
+        const int p = ok ? a.pos[from] : 0;
+        const unsigned move = __ballot_sync(0xffffffffu, ok);
+        constexpr int PARTS = D == 256 ? 2 : 1;          // 16-byte columns of K and V a lane has: D = 128 takes both in one go
+        uint4 v[B][PARTS];
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const long long f = __shfl_sync(0xffffffffu, from, b);
+#pragma unroll
+            for (int x = 0; x < PARTS; ++x) {
+                const __nv_bfloat16* base = PARTS == 2 ? (x ? a.v_pages : a.k_pages) : lane < 16 ? a.k_pages : a.v_pages;
+                if (move >> b & 1) v[b][x] = reinterpret_cast<const uint4*>(base + f * D)[PARTS == 2 ? lane : lane & 15];
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const long long t = __shfl_sync(0xffffffffu, to, b);
+#pragma unroll
+            for (int x = 0; x < PARTS; ++x) {
+                __nv_bfloat16* base = PARTS == 2 ? (x ? a.v_pages : a.k_pages) : lane < 16 ? a.k_pages : a.v_pages;
+                if (move >> b & 1) reinterpret_cast<uint4*>(base + t * D)[PARTS == 2 ? lane : lane & 15] = v[b][x];
+            }
+        }
+        if (ok) { a.mass[to] = m; a.pos[to] = p; }
     }
 }
 
@@ -396,9 +484,10 @@ int launch_mass(const MassArgs& a, int layers, cudaStream_t st) {
     }
     CUtensorMap map;
     if (!describe_rows(&map, a.k_pages, D, (unsigned long long)layers * a.num_pages * a.HK * kPage, (size_t)D * 2, 1, (size_t)D * 2, false, kPage, 1, 1)) return TF_ECUDA;
-    // blocks a column (layer, sequence, KV head): several rounds of the SMs, so that columns of unequal length even out
+    // Blocks a column (layer, sequence, KV head): one round of the SMs where that many columns fit it (64 columns of 4096 keys, 2 blocks: 30 us, 3:
+    // 39, 10: 37), a few otherwise, so that columns of unequal length even out (256 columns of 2048 to 8192 keys: 172 us with 1, 152 with 2, 149 with 3).
     const long long columns = (long long)layers * a.S * a.HK, tiles = (a.max_context + kMassKeys - 1) / kMassKeys;
-    const long long wanted = (4ll * kSms + columns - 1) / columns, blocks = wanted < tiles ? wanted : tiles;
+    const long long wanted = columns <= kSms ? kSms / columns : (3ll * kSms + columns - 1) / columns, blocks = wanted < tiles ? wanted : tiles;
     void* args[] = {const_cast<MassArgs*>(&a), &map};
     if (launch_pdl((const void*)mass_kernel<D>, dim3((unsigned)blocks, a.HK, layers * a.S), dim3(kMassThreads), C::SMEM, st, args) != cudaSuccess) {
         cudaGetLastError();
@@ -440,7 +529,7 @@ int tf_kv_evict(void* k_pages, void* v_pages, int num_pages, const int* page_tab
         return TF_EINVAL;
     if ((head_dim != 128 && head_dim != 256) || num_pages < 1 || max_pages < 1) return TF_EINVAL;
     if (!k_pages || !v_pages || !page_table || !seq_lens || !next_pos || !mass || !pos || !moved) return TF_EINVAL;
-    if (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15 || ((uintptr_t)mass | (uintptr_t)pos | (uintptr_t)moved | (uintptr_t)scratch) & 3) return TF_EALIGN;
+    if (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15 || ((uintptr_t)mass | (uintptr_t)pos) & 15 || ((uintptr_t)moved | (uintptr_t)scratch) & 3) return TF_EALIGN;
     if ((long long)layers * n_seqs > 65535 || kv_heads > 65535) return TF_EINVAL;
     if (!scratch || scratch_bytes < tf_evict_scratch_bytes(layers, n_seqs, kv_heads, budget, max_context)) return TF_ESCRATCH;
     const int most = max_context <= budget ? 1 : (max_context - budget < budget ? max_context - budget : budget);
@@ -464,7 +553,7 @@ int tf_kv_evict(void* k_pages, void* v_pages, int num_pages, const int* page_tab
         cudaGetLastError();
         return TF_ECUDA;
     }
-    const int blocks = min((most + tf::kMoveWarps - 1) / tf::kMoveWarps, 32);
+    const int blocks = min((most + 4 * tf::kMoveWarps - 1) / (4 * tf::kMoveWarps), 32);
     const void* move = head_dim == 256 ? (const void*)tf::evict_move_kernel<256> : (const void*)tf::evict_move_kernel<128>;
     if (tf::launch_pdl(move, dim3(blocks, kv_heads, layers * n_seqs), dim3(tf::kMoveWarps * 32), 0, st, args) != cudaSuccess) {
         cudaGetLastError();
