@@ -72,15 +72,18 @@ struct Ring {          // position in a ring of mbarrier-guarded slots
 };
 // Bounded waits of one role: after one that ran out (reported as TF_ESTALL) the others do not wait again, so that a kernel
 // whose pipeline broke ends at once, with its tensor memory given back.
+// The polls are one function for all waits: a kernel's roles share the SM's instruction cache.
+static __device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, int* status) {
+    for (int i = 0; i < 64; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
+    return mbar_wait_idle(bar, parity, status, 1000, 1 << 21);         // two seconds or so
+}
 struct Waits {
     int* status;
     bool dead = false;
     __device__ explicit Waits(int* s) : status(s) {}
     __device__ void operator()(uint32_t bar, uint32_t parity) {
-        if (dead) return;
-        for (int i = 0; i < 64; ++i)
-            if (mbar_try_wait(bar, parity)) return;
-        dead = !mbar_wait_idle(bar, parity, status, 1000, 1 << 21);        // two seconds or so
+        if (!mbar_try_wait(bar, parity) && !dead) dead = !wait_long(bar, parity, status);
     }
 };
 // Operand descriptors in two words. The low one holds the start address and the leading offset (in 16 bytes) and advances by constants,
@@ -148,6 +151,11 @@ __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// 16 bytes to shared memory, zeros where `read` is false (the source is not looked at then)
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool read) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
 }
 
 // ---- tiled copies --------------------------------------------------------------------------------------

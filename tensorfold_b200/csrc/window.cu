@@ -278,44 +278,42 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
                     }
                 }
                 if (!both) {
-                    // by the warp: lane takes 16-byte column `c` of one or two rows at a time; a page's loads before its first store
-                    constexpr int RPI = 32 / CPR, STEPS = kPage / RPI;
-                    const int c = lane % CPR;
-                    uint32_t bad = 0;
+                    // by the warp: lane takes 16-byte column `c` of one or two rows at a time, all on the way together. Bit r of `read`: the key
+                    // j0 + r is to be read (others become zeros); of `part`: some rows see it and some do not
+                    constexpr int RPI = 32 / CPR;
+                    const int c = lane % CPR, key = j0 + lane, first_new = w.L - j0;
+                    const bool wanted = !(lane < kPage ? copy[0] : copy[1]) && w.any_sees(key) && (lane >= first_new || (lane < kPage ? num[0] : num[1]) >= 0);
+                    const unsigned read = __ballot_sync(0xffffffffu, wanted);
+                    const unsigned part = __ballot_sync(0xffffffffu, wanted && !(key <= w.p_first && (key >= w.lo_last || key < w.sinks)));
+                    const __nv_bfloat16* from_new = src_new + ((ptrdiff_t)(w.r0 - first_new) * a.HK + w.kvh) * D + c * 8;
+                    uint8_t* const to = tile + (is_v ? half * 2 * C::PAGE_BYTES + (c >> 3) * (kPage * 128) : (c >> 3) * C::K_SLAB + half * 2 * (kPage * 128));
 #pragma unroll 1
                     for (int k = 0; k < 2; ++k) {
-                        if (k == 0 ? copy[0] : copy[1]) continue;
-                        const int number = k == 0 ? num[0] : num[1], key0 = j0 + k * kPage, pg = half * 2 + k;
-                        uint4 v[STEPS];
-#pragma unroll
-                        for (int x = 0; x < STEPS; ++x) {
-                            const int r = x * RPI + lane / CPR, key = key0 + r;
-                            v[x] = make_uint4(0, 0, 0, 0);
-                            if (!w.any_sees(key)) continue;
-                            if (key >= w.L) v[x] = *reinterpret_cast<const uint4*>(src_new + ((size_t)(w.r0 + key - w.L) * a.HK + w.kvh) * D + c * 8);
-                            else if (number >= 0)
-                                v[x] = *reinterpret_cast<const uint4*>(src_pages + (((size_t)number * a.HK + w.kvh) * kPage + r) * D + c * 8);
+                        if (k ? copy[1] : copy[0]) continue;
+                        const __nv_bfloat16* from_page = src_pages + ((size_t)max(k ? num[1] : num[0], 0) * a.HK + w.kvh) * (kPage * D) + c * 8;
+                        const uint32_t dst = smem_u32(to + k * (is_v ? C::PAGE_BYTES : kPage * 128));
+#pragma unroll 8
+                        for (int x = 0; x < kPage; x += RPI) {
+                            const int r = x + lane / CPR, at = k * kPage + r;
+                            cp_async16_or_zero(dst + r * 128 + (((c ^ r) & 7) << 4), at >= first_new ? from_new + (ptrdiff_t)at * a.HK * D : from_page + r * D, read >> at & 1);
                         }
-#pragma unroll
-                        for (int x = 0; x < STEPS; ++x) {
-                            const int r = x * RPI + lane / CPR;
-                            uint4 u = v[x];
-                            if (is_v) {                  // a value that is not finite: exponent all ones in either half
+                    }
+                    cp_async_commit();
+                    cp_async_wait<0>();
+                    uint32_t bad = 0;
+                    if (is_v) {
+                        for (unsigned left = part; left != 0; left &= left - 1) {
+                            const int at = __ffs(left) - 1, r = at & (kPage - 1);
+                            bool odd = false;
+                            uint4* cell = reinterpret_cast<uint4*>(to + (at >> 4) * C::PAGE_BYTES + r * 128 + (((c ^ r) & 7) << 4));
+                            if (lane / CPR == at % RPI) {            // the lanes that wrote it; a value that is not finite: exponent all ones in either half
+                                const uint4 u = *cell;
                                 const uint32_t e[4] = {u.x, u.y, u.z, u.w};
-                                bool odd = false;
 #pragma unroll
                                 for (int y = 0; y < 4; ++y) odd |= (e[y] & 0x7F80u) == 0x7F80u || (e[y] & 0x7F800000u) == 0x7F800000u;
-                                const unsigned m = __ballot_sync(0xffffffffu, odd);
-                                if (odd) u = make_uint4(0, 0, 0, 0);
-                                if (m) {
-#pragma unroll
-                                    for (int h = 0; h < RPI; ++h)
-                                        if (RPI == 1 || (m >> (h * 16) & 0xFFFFu) != 0) bad |= 1u << (k * kPage + x * RPI + h);
-                                }
-                                *reinterpret_cast<uint4*>(tile + pg * C::PAGE_BYTES + (c >> 3) * (kPage * 128) + r * 128 + (((c ^ r) & 7) << 4)) = u;
-                            } else {
-                                *reinterpret_cast<uint4*>(tile + (c >> 3) * C::K_SLAB + (pg * kPage + r) * 128 + (((c ^ r) & 7) << 4)) = u;
+                                if (odd) *cell = make_uint4(0, 0, 0, 0);
                             }
+                            if (__any_sync(0xffffffffu, odd)) bad |= 1u << at;
                         }
                     }
                     if (is_v && lane == 0) bad_s[ring.i * 2 + half] = bad;
@@ -430,8 +428,12 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_empty(b));
                 if (!plain) {                            // the V tile's notes are there once it is (and stay until P V)
-                    wait(v_full(vr.i), vr.phase);
-                    const uint32_t bad[2] = {bad_s[vr.i * 2], bad_s[vr.i * 2 + 1]};
+                    uint32_t bad[2] = {0, 0};
+                    if (w.p_first != w.p_last) {         // (a row alone sees all that is read)
+                        wait(v_full(vr.i), vr.phase);
+                        bad[0] = bad_s[vr.i * 2];
+                        bad[1] = bad_s[vr.i * 2 + 1];
+                    }
                     // bit e: the row sees key j0 + e; up to p, and from lo on or below the sinks' end
                     auto below = [](int x) -> unsigned long long { return x <= 0 ? 0ull : x >= kTile ? ~0ull : (1ull << x) - 1; };
                     const unsigned long long sees = below(p + 1 - j0) & (~below(lo - j0) | below(w.sinks - j0));
