@@ -56,6 +56,8 @@ struct WindowArgs {
     int chunk, first_slots, near_slots, slots;         // keys a chunk; slots of the sinks' chunks, of the window's, of both
     int qgroups, group_rows, items;                    // groups of window rows, rows a group; (group, slot, KV head, sequence) in all
     FastDiv by_group, by_slot, by_head, by_G, by_chunk;
+    int* plan;                         // [rounds, kSms] items by block, -1: none; null: block b takes items b, b + blocks, ...
+    int rounds;
     float scale_log2;
 };
 
@@ -75,18 +77,21 @@ __host__ __device__ inline Slots slots_for(int window, int sinks, int max_window
 __device__ __forceinline__ int slot_of(int chunk, int first, int near) { return chunk < first ? chunk : first + (chunk - first) % near; }
 
 // The sequence that holds packed row `row`: the last one that starts at or before it (a sequence without rows starts where the
-// next one does, and is passed over); -1 for a row behind the last sequence. Whole warps.
-__device__ __forceinline__ int seq_of(const int* seq_start, int S, int row) {
+// next one does, and is passed over), and where it starts; -1 for a row behind the last sequence. Whole warps; one load for up to 31
+// sequences.
+__device__ __forceinline__ int seq_of(const int* seq_start, int S, int row, int& start) {
     const int lane = threadIdx.x & 31;
-    if (row >= seq_start[S]) return -1;
     int found = -1;
-    for (int s0 = 0; s0 < S; s0 += 32) {
-        const bool before = s0 + lane < S && seq_start[s0 + lane] <= row;
-        const unsigned m = __ballot_sync(0xffffffffu, before);
-        if (m) found = s0 + 31 - __clz(m);
+    for (int s0 = 0; s0 <= S; s0 += 32) {
+        const int v = s0 + lane <= S ? seq_start[s0 + lane] : 0x7FFFFFFF;
+        const unsigned m = __ballot_sync(0xffffffffu, v <= row);
+        if (m) {
+            found = s0 + 31 - __clz(m);
+            start = __shfl_sync(0xffffffffu, v, 31 - __clz(m));
+        }
         if (m != 0xffffffffu) break;
     }
-    return found;
+    return found >= S ? -1 : found;              // at or behind seq_start[S]
 }
 
 // One chunk of one (sequence, KV head) for one group of window rows; every role of a block forms it by itself.
@@ -105,12 +110,11 @@ struct Work {
     }
     __device__ bool any_sees(int j) const { return j <= p_last && (j >= lo_first || j < sinks); }
 };
-struct Raw {           // what a block's next item needs from memory, fetched while the one before it is worked on
+struct Raw {           // what an item needs from memory
     int r0, r1, L;
 };
-// The row groups of one chunk are neighbours: they read the same keys at the same time.
 __device__ __forceinline__ Raw fetch(const WindowArgs& a, int item) {
-    if (item >= a.items) return {0, 0, 0};
+    if (item < 0) return {0, 0, 0};
     const int seq = a.by_head(a.by_slot(a.by_group(item)));
     return {a.seq_start[seq], a.seq_start[seq + 1], a.seq_lens[seq]};
 }
@@ -150,6 +154,76 @@ __device__ __forceinline__ Work work_of(const WindowArgs& a, int item, Raw raw, 
     w.far_tile = max(w.head_tiles, w.lo_first > w.key0 ? (w.lo_first - w.key0) / kTile : 0);
     w.tiles = w.head_tiles + max(0, in_chunk - w.far_tile);
     return w;
+}
+
+// A role's walk over its block's items. What the next one needs is fetched while the one before it is worked on.
+struct Walk {
+    int item, next, k = 0;
+    Raw raw;
+    __device__ explicit Walk(const WindowArgs& a) : item(at(a, 0)), next(at(a, 1)), raw(fetch(a, item)) {}
+    __device__ static int at(const WindowArgs& a, int k) {
+        if (a.plan != nullptr) return k < a.rounds ? a.plan[k * kSms + blockIdx.x] : -1;
+        const int i = blockIdx.x + k * gridDim.x;
+        return i < a.items ? i : -1;
+    }
+    __device__ Work work(const WindowArgs& a, bool speaks) {
+        const Work w = work_of(a, item, raw, speaks);
+        raw = fetch(a, next);
+        return w;
+    }
+    __device__ void step(const WindowArgs& a) {
+        item = next;
+        next = at(a, ++k + 1);
+    }
+};
+
+// Which block takes which items, where a block takes several: the items that have work, by falling weight, dealt out back and forth, so that
+// the blocks end together (16 users: 40 tiles of 64 keys on the busiest block without it, 28 on average). One block; the
+// order among equals does not matter, no item's result depends on where it runs.
+constexpr int kPlanThreads = 1024, kPlanItems = 8192, kPlanBins = 128;
+constexpr size_t kPlanBytes = ((kPlanItems + kSms - 1) / kSms * kSms * sizeof(int) + 255) / 256 * 256;
+__global__ void __launch_bounds__(kPlanThreads) window_plan_kernel(const WindowArgs a) {
+    __shared__ int count[kPlanBins], start[kPlanBins];
+    pdl_launch_dependents();
+    const int tid = threadIdx.x;
+    if (tid < kPlanBins) count[tid] = 0;
+    pdl_wait();                                  // the plan may still be the one of a call before this
+    for (int i = tid; i < a.rounds * kSms; i += kPlanThreads) a.plan[i] = -1;
+    __syncthreads();
+    constexpr int PER = kPlanItems / kPlanThreads;
+    int place[PER];                              // bin << 16 | rank in it
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int item = tid + k * kPlanThreads;
+        place[k] = -1;
+        if (item >= a.items) continue;
+        const int tiles = work_of(a, item, fetch(a, item), true).tiles;
+        if (tiles == 0) continue;
+        const int bin = kPlanBins - 1 - min(tiles, kPlanBins - 1);
+        place[k] = bin << 16 | atomicAdd(&count[bin], 1);
+    }
+    __syncthreads();
+    if (tid < 32) {
+        int before = 0;
+        for (int b0 = 0; b0 < kPlanBins; b0 += 32) {
+            const int c = count[b0 + tid];
+            int x = c;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (tid >= o) x += y;
+            }
+            start[b0 + tid] = before + x - c;
+            before += __shfl_sync(0xffffffffu, x, 31);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        if (place[k] < 0) continue;
+        const int at = start[place[k] >> 16] + (place[k] & 0xFFFF), round = at / kSms, in_round = at - round * kSms;
+        a.plan[round * kSms + (round & 1 ? kSms - 1 - in_round : in_round)] = tid + k * kPlanThreads;
+    }
 }
 
 template <int D, int QR>
@@ -219,8 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
     pdl_wait();
 
     // All roles go through the block's items and their tiles in the same order and keep step by barriers: nobody is more than a ring ahead.
-    int item = blockIdx.x;
-    Raw raw = fetch(a, item);
+    Walk walk(a);
     if (warp >= kKWarp) {
         // ------------------------------- producers: two warps for K, two for V, half a tile each -----------------------
         const bool is_v = warp >= kVWarp;
@@ -231,9 +304,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
         const uint32_t full0 = is_v ? v_full(0) : k_full(0), empty0 = is_v ? v_empty(0) : k_empty(0);
         if (lane == 0) { tma_prefetch_map(pages); tma_prefetch_map(rows); }
         Ring ring(is_v ? VS : KS, 1);
-        for (; item < a.items; item += gridDim.x) {
-            const Work w = work_of(a, item, raw, false);
-            raw = fetch(a, item + gridDim.x);
+        for (; walk.item >= 0; walk.step(a)) {
+            const Work w = walk.work(a, false);
             const int* pt = a.page_table + (size_t)w.seq * a.max_pages;
             // page numbers of eight tiles at a time, a lane each, a batch ahead
             auto numbers = [&](int i) -> int {
@@ -327,9 +399,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
     } else if (warp == kQWarp) {
         // ------------------------------- Q: row = t * G + head, once an item -------------------------------------------
         Ring ring(1, 1);
-        for (; item < a.items; item += gridDim.x) {
-            const Work w = work_of(a, item, raw, false);
-            raw = fetch(a, item + gridDim.x);
+        for (; walk.item >= 0; walk.step(a)) {
+            const Work w = walk.work(a, false);
             if (w.tiles == 0) continue;
             wait(q_empty, ring.phase);
             ring.next();
@@ -350,9 +421,9 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
         const uint32_t q_lo = desc_lo(smem_u32(q_s), 1);
         Ring kr(KS, 0), vr(VS, 0), qr(1, 0);
         int it = 0;                                      // tiles so far, over all items
-        for (; item < a.items; item += gridDim.x) {
-            const int tiles = __reduce_max_sync(0xffffffffu, work_of(a, item, raw, false).tiles);
-            raw = fetch(a, item + gridDim.x);
+        for (;; walk.step(a)) {
+            const int tiles = __reduce_max_sync(0xffffffffu, walk.item >= 0 ? walk.work(a, false).tiles : -1);
+            if (tiles < 0) break;
             if (tiles == 0) continue;
             wait(q_full, qr.phase);
             qr.next();
@@ -397,9 +468,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
         const unsigned long long scale2 = pair_of(a.scale_log2, a.scale_log2);
         Ring vr(VS, 0);
         int it = 0;
-        for (; item < a.items; item += gridDim.x) {
-            const Work w = work_of(a, item, raw, tid == 0);
-            raw = fetch(a, item + gridDim.x);
+        for (; walk.item >= 0; walk.step(a)) {
+            const Work w = walk.work(a, tid == 0);
             if (w.tiles == 0) continue;
             if (warp * 32 >= w.nq) {                     // no rows: keeps step with the others, tile by tile
                 for (int i = 0; i < w.tiles; ++i, ++it, vr.next()) {
@@ -543,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
 
 // Joins the chunks of a row, in order: D / 8 lanes a (row, head), eight values a lane. Chunks in which the row sees nothing are
 // passed over, so the join does not depend on which chunks the rows beside it needed.
-template <int D>
+template <int D, int B>
 __global__ void __launch_bounds__(128) window_join_kernel(const WindowArgs a) {
     constexpr int LANES = D / 8, PER_WARP = 32 / LANES;
     pdl_launch_dependents();
@@ -551,7 +621,8 @@ __global__ void __launch_bounds__(128) window_join_kernel(const WindowArgs a) {
     const int row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int head = (blockIdx.x * 4 + warp) * PER_WARP + lane / LANES, li = lane % LANES;
     const int Mp = tf_padded_rows(a.R);
-    const int seq = row < a.R ? seq_of(a.seq_start, a.S, row) : -1;
+    int start = 0;
+    const int seq = row < a.R ? seq_of(a.seq_start, a.S, row, start) : -1;
     const bool there = head < a.H;
     const int c8 = head * LANES + li;
     if (seq < 0) {
@@ -561,7 +632,7 @@ __global__ void __launch_bounds__(128) window_join_kernel(const WindowArgs a) {
         }
         return;
     }
-    const int p = a.seq_lens[seq] + row - a.seq_start[seq];
+    const int p = a.seq_lens[seq] + row - start;
     if (p < 0 || p >= a.max_context) return;                           // reported by the chunk kernel
     const int lo = max(0, p + 1 - a.window);
     // chunks with sinks below the window, then the window's
@@ -570,16 +641,18 @@ __global__ void __launch_bounds__(128) window_join_kernel(const WindowArgs a) {
     float acc[8], m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-    constexpr int B = 4;                                               // chunks whose loads are in flight together
+    // B: chunks whose loads are in flight together
     for (int i0 = 0; i0 < count; i0 += B) {
         float cm[B], cl[B];
         float4 po[B][2];
 #pragma unroll
         for (int k = 0; k < B; ++k) {
-            const int i = min(i0 + k, count - 1), chunk = i < head_chunks ? i : far + i - head_chunks;
+            cl[k] = 0.f;
+            if (i0 + k >= count) continue;
+            const int i = i0 + k, chunk = i < head_chunks ? i : far + i - head_chunks;
             const size_t cell = ((size_t)slot_of(chunk, a.first_slots, a.near_slots) * a.R + row) * a.H + (there ? head : 0);
             cm[k] = a.part_m[cell];
-            cl[k] = i0 + k < count ? a.part_l[cell] : 0.f;
+            cl[k] = a.part_l[cell];
             const float4* src = reinterpret_cast<const float4*>(a.part_o + cell * D + li * 8);
             po[k][0] = src[0];
             po[k][1] = src[1];
@@ -657,11 +730,19 @@ int run(WindowArgs& a, cudaStream_t st) {
     if (items > (1 << 30)) return TF_EINVAL;
     a.items = (int)items;
     a.by_group = fast_div(a.qgroups); a.by_slot = fast_div(a.slots); a.by_head = fast_div(a.HK); a.by_G = fast_div(G); a.by_chunk = fast_div(a.chunk);
+    a.rounds = (a.items + kSms - 1) / kSms;
+    if (a.rounds < 2 || a.items > kPlanItems) a.plan = nullptr;        // one item a block at most; so many that they even out
+    if (a.plan != nullptr) {
+        void* args[] = {&a};
+        if (launch_pdl((const void*)window_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, args) != cudaSuccess) { cudaGetLastError(); return TF_ECUDA; }
+    }
     const int rc = a.group_rows * G <= 64 ? launch_chunks<D, 64>(a, st) : launch_chunks<D, 128>(a, st);
     if (rc != TF_OK) return rc;
     void* join[] = {&a};
     const int heads = 4 * (32 / (D / 8)), out_rows = a.out_packed ? tf_padded_rows(a.R) : a.R;
-    if (launch_pdl((const void*)window_join_kernel<D>, dim3((a.H + heads - 1) / heads, out_rows), dim3(128), 0, st, join) != cudaSuccess) {
+    // (one row of 7 chunks: 11.3 us with eight in flight, 12 with four; 2900 rows of one or two: 14 and 24 us for this kernel)
+    const void* kern = a.slots > 4 ? (const void*)window_join_kernel<D, 8> : (const void*)window_join_kernel<D, 4>;
+    if (launch_pdl(kern, dim3((a.H + heads - 1) / heads, out_rows), dim3(128), 0, st, join) != cudaSuccess) {
         cudaGetLastError();
         return TF_ECUDA;
     }
@@ -682,7 +763,7 @@ int tf_window_slots(int window, int sinks, int max_window, int max_context, int 
 
 size_t tf_window_scratch_bytes(int rows, int heads, int head_dim, int slots) {
     if (rows < 1 || heads < 1 || head_dim < 1 || slots < 1) return 0;
-    return (size_t)slots * rows * heads * (head_dim + 2) * sizeof(float);
+    return tf::kPlanBytes + (size_t)slots * rows * heads * (head_dim + 2) * sizeof(float);
 }
 
 int tf_window_attention(const void* q, const void* k_new, const void* v_new, const void* k_pages, const void* v_pages, int num_pages,
@@ -717,7 +798,8 @@ int tf_window_attention(const void* q, const void* k_new, const void* v_new, con
     const tf::Slots cut = tf::slots_for(window, sinks, max_window, max_context, chunk_keys);
     a.first_slots = cut.first; a.near_slots = cut.near > 0 ? cut.near : 1;
     const size_t cells = (size_t)slots * rows * heads;
-    a.part_o = static_cast<float*>(scratch);
+    a.plan = static_cast<int*>(scratch);
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(scratch) + tf::kPlanBytes);
     a.part_m = a.part_o + cells * head_dim;
     a.part_l = a.part_m + cells;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
