@@ -312,7 +312,9 @@ int tf_lane_attention_paged_static(const void* q, const void* k_new, const void*
  * stands at slot p = seq_lens[s] + t and sees key j <= p where p - j < window or j < sinks; window 0: every key up to its own
  * (sinks then change nothing). Keys are cut by absolute position into chunks of chunk_keys (a multiple of 64) that are
  * attended by themselves and joined in order, so a row's bits depend on chunk_keys and on its own keys only. A call's partials
- * live in `slots` = tf_window_slots(...) chunks of scratch (tf_window_scratch_bytes). num_pages bounds the page numbers: an entry
+ * live in `slots` = tf_window_slots(...) chunks of scratch (tf_window_scratch_bytes, 16-byte aligned, no initialisation; calls that overlap
+ * on the GPU must not share it). tf_window_launches: how many kernels a call queues: the chunks and the join, before them a plan where
+ * blocks take several chunks. q, k_new, v_new, pages, out 16-byte aligned. num_pages bounds the page numbers: an entry
  * outside [0, num_pages) on a page that a row sees is reported as TF_EINVAL through `status` and its keys are left out; entries of
  * pages that no row sees are not read. max_window bounds a sequence's rows, max_context its keys with its window's own (also
  * reported). lse, when not NULL, receives ln(sum exp(score)) [rows, heads] fp32. Rows behind seq_start[n_seqs] are left as
@@ -320,6 +322,7 @@ int tf_lane_attention_paged_static(const void* q, const void* k_new, const void*
  * rows of a page, later rows) may hold anything; a row that sees a value that is not finite has no specified result. */
 int tf_window_slots(int window, int sinks, int max_window, int max_context, int chunk_keys);
 size_t tf_window_scratch_bytes(int rows, int heads, int head_dim, int slots);
+int tf_window_launches(int rows, int n_seqs, int max_window, int slots, int heads, int kv_heads);
 int tf_window_attention(const void* q, const void* k_new, const void* v_new, const void* k_pages, const void* v_pages, int num_pages,
                         const int* page_table, int max_pages, const int* seq_lens, const int* seq_start, void* out, float* lse,
                         const void* qg, size_t qg_stride, void* out_packed, int group, void* scratch, size_t scratch_bytes, int rows,
@@ -340,14 +343,14 @@ int tf_kv_commit(const void* k_new, const void* v_new, long long rec_stride, voi
  *   query heads of exp(scale q . k_j - lse), in row order; keys that the commit brought start at that sum and their pos becomes
  *   row_pos of their row. q [layers, rows, heads, D] bf16 and lse [layers, rows, heads] fp32 are the attention's queries and
  *   log-sum-exps; k_pages [layers, num_pages, kv_heads, 16, D]; mass fp32 and pos int32 [layers, num_pages, kv_heads, 16].
- *   A sequence with keep 0 is left as it was.
+ *   A sequence with keep 0 is left as it was. q, k_pages 16-byte aligned.
  * tf_kv_evict: every sequence of more than `budget` slots is cut back to it, each (layer, KV head) by itself. Kept are the slots
  *   with pos < sinks or pos >= next_pos[s] - recent, then those of the largest mass (ties to the lower slot, NaN counts as -inf); the i-th kept slot
  *   at or above the budget moves into the i-th evicted one below it (K, V, mass, pos), the other slots are not touched. moved
  *   [layers, n_seqs, kv_heads] receives how many moved. seq_lens is not written: the caller's sequences now have
- *   min(length, budget) slots, whose order no longer follows the text. Pages must belong to one sequence only.
- *   scratch: tf_evict_scratch_bytes, 4-byte aligned, no initialisation; two launches.
- * Both report a page number outside [0, num_pages) or a length above max_context as TF_EINVAL through `status` and leave those slots out. */
+ *   min(length, budget) slots, whose order no longer follows the text.
+ *   k_pages, v_pages, mass, pos 16-byte aligned. scratch: tf_evict_scratch_bytes, 4-byte aligned, no initialisation; two launches.
+ * Calls that overlap on the GPU must not share a cache or scratch; a page belongs to one sequence. Both report a page number outside [0, num_pages) or a length above max_context as TF_EINVAL through `status` and leave those slots out. */
 int tf_attention_mass(const void* q, const float* lse, const void* k_pages, int num_pages, const int* page_table, int max_pages,
                       const int* seq_lens, const int* seq_start, const int* keep, const int* row_pos, float* mass, int* pos, int layers,
                       int rows, int n_seqs, int max_window, int max_context, int heads, int kv_heads, int head_dim, float scale, int* status,

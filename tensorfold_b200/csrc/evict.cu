@@ -63,7 +63,6 @@ __global__ void __launch_bounds__(kMassThreads, 1) mass_kernel(const __grid_cons
     auto s_full = [&](int s) { return bars + 8u * (2 * KS + s); };
     auto s_empty = [&](int s) { return bars + 8u * (2 * KS + 2 + s); };
     const uint32_t q_full = bars + 8u * (2 * KS + 4), q_empty = q_full + 8;
-    pdl_launch_dependents();
     pdl_wait();
     // ---- the block's share of the tiles of (layer, sequence, KV head) ----
     const int kvh = blockIdx.y, layer = blockIdx.z / a.S, seq = blockIdx.z - layer * a.S, G = a.H / a.HK;
@@ -88,6 +87,7 @@ __global__ void __launch_bounds__(kMassThreads, 1) mass_kernel(const __grid_cons
     if (warp == kMassMma) tc_alloc(smem_u32(&tmem_s), 2 * kMassRows);
     tc_fence_before();
     __syncthreads();
+    pdl_launch_dependents();        // not before the tensor memory is this block's: a dependent that held it would wait for this kernel
     tc_fence_after();
     const uint32_t tmem = tmem_s;
     Waits wait(a.status);

@@ -351,7 +351,7 @@ PyObject* window_attention_py(PyObject* const* args, Py_ssize_t n) {
                                    (int)d, (float)scale, status, stream.stream());
     }();
     check_rc(rc, "window_attention");
-    g_launches.fetch_add(2, std::memory_order_relaxed);
+    g_launches.fetch_add(tf_window_launches((int)r, (int)s, max_window, slots, (int)h, (int)hk), std::memory_order_relaxed);
     if (!out.defined()) Py_RETURN_NONE;
     return THPVariable_Wrap(out);
 }
@@ -506,7 +506,8 @@ PyMethodDef methods[] = {
     TF_FN(tf_moe_combine_peer, 1), TF_FN(tf_moe_pack, 1), TF_FN(tf_moe_act, 1), TF_FN(tf_moe_combine, 1), TF_FN(tf_peer_slot_bytes, 0),
     TF_FN(tf_peer_exchange, 1), TF_FN(tf_qmm_act, 1), TF_FN(tf_swiglu_tiled, 1), TF_FN(tf_qmm_peer, 1), TF_FN(tf_norm_xs_peer, 1),
     TF_FN(tf_set_poll_limit, 0), TF_FN(tf_topk_scratch_bytes, 0), TF_FN(tf_topk_rows, 2), TF_FN(tf_topk_sample_rows, 2), TF_FN(tf_sample_rows, 1),
-    TF_FN(tf_window_slots, 0), TF_FN(tf_window_scratch_bytes, 0), TF_FN(tf_window_attention, 2), TF_FN(tf_attention_mass, 1),
+    TF_FN(tf_window_slots, 0), TF_FN(tf_window_scratch_bytes, 0), TF_FN(tf_window_launches, 0),
+    TF_FN(tf_window_attention, 2), TF_FN(tf_attention_mass, 1),        // (without a plan; window_attention() counts it)
     TF_FN(tf_evict_scratch_bytes, 0), TF_FN(tf_kv_evict, 2), TF_FN(tf_verify_scratch_bytes, 0), TF_FN(tf_verify_rows, 2),
     TF_OWN("bound", bound_py), TF_OWN("scratch", scratch_py), TF_OWN("lane_matmul", lane_matmul_py), TF_OWN("prefill_matmul", prefill_matmul_py),
     TF_OWN("window_attention", window_attention_py), TF_OWN("attention_mass", attention_mass_py), TF_OWN("evict", evict_py),

@@ -720,18 +720,26 @@ int launch_chunks(const WindowArgs& a, cudaStream_t st) {
     return TF_OK;
 }
 
-template <int D>
-int run(WindowArgs& a, cudaStream_t st) {
-    const int G = a.H / a.HK, most = kRows / G;
+// Rows a group, groups of rows and items of a call; false where the items are more than the launch can count.
+bool cut_rows(WindowArgs& a) {
+    const int most = kRows / (a.H / a.HK);
     a.group_rows = a.max_window < most ? a.max_window : most;
     if (a.group_rows > a.R) a.group_rows = a.R;
     a.qgroups = (a.max_window + a.group_rows - 1) / a.group_rows;
     const long long items = (long long)a.qgroups * a.slots * a.HK * a.S;
-    if (items > (1 << 30)) return TF_EINVAL;
     a.items = (int)items;
+    return items <= (1 << 30);
+}
+// A plan only where a block takes several items, and not so many that they even out.
+bool planned(int items) { return items > kSms && items <= kPlanItems; }
+
+template <int D>
+int run(WindowArgs& a, cudaStream_t st) {
+    const int G = a.H / a.HK;
+    if (!cut_rows(a)) return TF_EINVAL;
     a.by_group = fast_div(a.qgroups); a.by_slot = fast_div(a.slots); a.by_head = fast_div(a.HK); a.by_G = fast_div(G); a.by_chunk = fast_div(a.chunk);
     a.rounds = (a.items + kSms - 1) / kSms;
-    if (a.rounds < 2 || a.items > kPlanItems) a.plan = nullptr;        // one item a block at most; so many that they even out
+    if (!planned(a.items)) a.plan = nullptr;
     if (a.plan != nullptr) {
         void* args[] = {&a};
         if (launch_pdl((const void*)window_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, args) != cudaSuccess) { cudaGetLastError(); return TF_ECUDA; }
@@ -764,6 +772,13 @@ int tf_window_slots(int window, int sinks, int max_window, int max_context, int 
 size_t tf_window_scratch_bytes(int rows, int heads, int head_dim, int slots) {
     if (rows < 1 || heads < 1 || head_dim < 1 || slots < 1) return 0;
     return tf::kPlanBytes + (size_t)slots * rows * heads * (head_dim + 2) * sizeof(float);
+}
+
+int tf_window_launches(int rows, int n_seqs, int max_window, int slots, int heads, int kv_heads) {
+    if (rows < 1 || n_seqs < 1 || max_window < 1 || slots < 1 || kv_heads < 1 || heads < kv_heads || heads / kv_heads > 16) return 0;
+    tf::WindowArgs a{};
+    a.R = rows; a.S = n_seqs; a.max_window = max_window; a.slots = slots; a.H = heads; a.HK = kv_heads;
+    return !tf::cut_rows(a) ? 0 : tf::planned(a.items) ? 3 : 2;
 }
 
 int tf_window_attention(const void* q, const void* k_new, const void* v_new, const void* k_pages, const void* v_pages, int num_pages,

@@ -20,6 +20,7 @@ import torch
 from .exact_sampling import Sampling, sample_rows
 from .forward import State, Weights, accept_path, commit, tree_forward
 from .lane_qmm import MAX_ROWS, lane_matmul
+from .speculative import verify_drafts
 
 
 @dataclass
@@ -141,7 +142,7 @@ def serial_decode(w: Weights, st: State, pending: Sequence[int], count: int, sam
     rounds = 0
     while len(out[0]) < count:
         logits, rec = tree_forward(w, _tokens([o[-1] for o in out], dev), [1] * n, st)
-        nxt = sample_rows(logits, [st.lens[s] + 1 for s in range(n)], sampling).tolist()
+        nxt = sample_rows(logits, [st.position(s) + 1 for s in range(n)], sampling).tolist()
         commit(st, rec, [1] * n)
         for s in range(n):
             out[s].append(int(nxt[s]))
@@ -186,7 +187,7 @@ def draft_decode(w: Weights, st: State, prompts: Sequence[Sequence[int]], pendin
         widths = [len(wd) for wd in windows]
         rows = [t for wd in windows for t in wd]
         logits, rec = tree_forward(w, _tokens(rows, dev), widths, st)
-        positions = [st.lens[s] + t + 1 for s in range(n) for t in range(widths[s])]
+        positions = [st.position(s) + t + 1 for s in range(n) for t in range(widths[s])]
         verified = sample_rows(logits, positions, sampling).tolist()
         keep, r = [], 0
         for s in range(n):
@@ -209,26 +210,98 @@ def draft_decode(w: Weights, st: State, prompts: Sequence[Sequence[int]], pendin
     return DecodeResult([o[:count] for o in out], time.perf_counter() - start, rounds, drafted, accepted, widths_log)
 
 
+@torch.no_grad()
+def sampled_decode(w: Weights, st: State, prompts: Sequence[Sequence[int]], pending: Sequence[int], count: int, *, temperature: float = 1.0,
+                   generator: torch.Generator | None = None, max_rows: int = 8, draft: Callable | None = None,
+                   draft_temperature: float | None = None) -> DecodeResult:
+    """``draft_decode`` with drafts that are kept by chance: a guess x that the drafter drew with probability q(x) is kept with probability
+    min(1, p(x) / q(x)), p the target's distribution at ``temperature`` over the whole vocabulary, and the first refused one is replaced by a draw from
+    max(p - q, 0) (``speculative.verify_drafts``): the tokens are distributed as serial sampling's, whatever the drafter proposes.
+
+    ``draft(seq, context, k)`` returns up to k guesses, or (guesses, logits) with the (guesses, vocabulary) logits that they were drawn from
+    at ``draft_temperature`` (default: ``temperature``); guesses without logits, and the n-gram copies of the default drafter, are
+    taken as certain (q = 1). ``generator``: of the uniform random numbers, on the weights' device.
+    """
+
+    if count < 1 or not 1 <= max_rows <= MAX_ROWS:
+        raise ValueError(f"count >= 1 and 1 <= max_rows <= {MAX_ROWS} required")
+    dev = w.norm.device
+    n = st.n_seqs
+    out = [[int(p)] for p in pending]
+    context = [list(prompts[s]) + out[s] for s in range(n)]
+    copies = [CopyIndex() for _ in range(n)]
+    rounds = drafted = accepted = 0
+    widths_log = []
+    start = time.perf_counter()
+    while any(len(o) < count for o in out):
+        budget = max(1, MAX_ROWS // max(1, sum(len(o) < count for o in out)))
+        rows, widths, given = [], [], []
+        for s in range(n):
+            if len(out[s]) >= count:
+                widths.append(0)
+                continue
+            k = max(min(max_rows, budget, count - len(out[s])) - 1, 0)
+            made = draft(s, context[s], k) if draft is not None else copies[s].propose(context[s], k)
+            guesses, logits = made if isinstance(made, tuple) else (made, None)
+            guesses = [int(g) for g in guesses][:k]
+            if any(not 0 <= g < w.config.vocab for g in guesses):
+                raise ValueError("sampled_decode: draft returned a token outside the vocabulary")
+            if logits is not None and (logits.dim() != 2 or logits.shape[0] < len(guesses) or logits.shape[1] != w.config.vocab):
+                raise ValueError("sampled_decode: draft's logits must be (guesses, vocabulary)")
+            if logits is not None and guesses:
+                given.append((len(rows) + 1, len(guesses), logits))
+            rows += [out[s][-1]] + guesses
+            widths.append(1 + len(guesses))
+        tokens = _tokens(rows, dev)
+        logits, rec = tree_forward(w, tokens, widths, st)
+        near = None
+        if given:                              # guesses without logits beside some with: all of q on the guess
+            near = torch.full_like(logits, float("-inf"))
+            near.scatter_(1, tokens.long().unsqueeze(1), 0.0)
+            for first, many, theirs in given:
+                near[first:first + many] = theirs[:many]
+        uniforms = torch.rand((len(rows), 2), generator=generator, device=dev)
+        keep, token = verify_drafts(logits, tokens, rec.batch.seq_start, uniforms, temperature=temperature, draft_logits=near,
+                                    draft_temperature=draft_temperature)
+        keep, token = torch.stack([keep, token]).tolist()
+        r = 0
+        for s in range(n):
+            if widths[s]:
+                new = rows[r + 1:r + keep[s]] + [token[s]]
+                out[s].extend(new)
+                context[s].extend(new)
+                drafted += widths[s] - 1
+                accepted += keep[s] - 1
+            r += widths[s]
+        commit(st, rec, keep)
+        rounds += 1
+        widths_log.append(sum(widths))
+    torch.cuda.synchronize(dev)
+    return DecodeResult([o[:count] for o in out], time.perf_counter() - start, rounds, drafted, accepted, widths_log)
+
+
 class Engine:
     """The engine contract the reference's server drives (``cuda/server.py:9-15``): ``eos`` and
     ``generate(prompt, max_tokens, sampling, on_tokens) -> dict`` for one request at a time, decoded as one
     exact stream: prefill through the lane forward, then drafted rounds (n-gram copy drafter) whose output is
     token for token what serial decoding gives. A prompt that extends the previous request's reuses its
     committed state (``State.snapshot`` / ``restore`` at the end of the shared prefix is the caller's tool for
-    anything finer). ``prompt_rows``: rows of a prompt processed in one pass, fewer where memory is short."""
+    anything finer). ``prompt_rows``: rows of a prompt processed in one pass, fewer where memory is short. ``window``, ``sinks``, ``budget``,
+    ``recent``: how the state bounds its attention (``State``; with a budget, drafted rounds are not token for token serial decoding)."""
 
     def __init__(self, w: Weights, *, max_context: int = 8192, eos: Sequence[int] = (), max_rows: int = 8,
-                 prompt_rows: int = PROMPT_ROWS):
+                 prompt_rows: int = PROMPT_ROWS, window: int | None = None, sinks: int = 0, budget: int | None = None, recent: int = 0):
         if not 1 <= prompt_rows <= MAX_ROWS:
             raise ValueError(f"1 <= prompt_rows <= {MAX_ROWS} required")
         self.prompt_rows = prompt_rows
         self.w, self.eos, self.max_rows, self.max_context = w, tuple(int(t) for t in eos), max_rows, max_context
-        self.state = State(w, 1, max_context)
+        self.bounds = dict(window=window, sinks=sinks, budget=budget, recent=recent)
+        self.state = State(w, 1, max_context, **self.bounds)
         self.committed: list = []              # tokens whose state is committed
 
     def _reset(self) -> None:
         self.state.kv.release(0)
-        self.state = State(self.w, 1, self.max_context)
+        self.state = State(self.w, 1, self.max_context, **self.bounds)
         self.committed = []
 
     def generate(self, prompt: Sequence[int], max_tokens: int, sampling: Sampling | None = None,
@@ -266,4 +339,4 @@ class Engine:
         return {"tokens": out[:max_tokens], "seconds": time.perf_counter() - start, "rounds": rounds, "prompt_tokens": len(prompt)}
 
 
-__all__ = ["CopyIndex", "DecodeResult", "Engine", "draft_decode", "prefill", "serial_decode"]
+__all__ = ["CopyIndex", "DecodeResult", "Engine", "draft_decode", "prefill", "sampled_decode", "serial_decode"]

@@ -18,7 +18,7 @@ from typing import Sequence
 import torch
 
 from . import lane_attention as LA
-from . import lane_gdn, lane_glue
+from . import lane_evict, lane_gdn, lane_glue, lane_window
 from . import lane_moe
 from .lane_qmm import MAX_ROWS, QWeight, new_packed, tile_weight
 from .lane_qmm import lane_matmul as _lane_matmul
@@ -196,12 +196,29 @@ def load_weights(model: dict, device="cuda") -> Weights:
 class State:
     """Committed state of ``n_seqs`` sequences: paged K/V for the attention layers, conv tail and fp32
     recurrent state for the GDN layers, and each sequence's committed length. Read-only during a
-    forward; only ``commit`` writes it (reference: ``forward.State``)."""
+    forward; only ``commit`` writes it (reference: ``forward.State``).
+
+    Two ways to bound what a sequence's attention costs (no counterpart in the reference); a state has one of them or neither, in
+    all its steps. ``window``: attention layers see the ``window`` latest positions and the first ``sinks`` ones (``lane_window``), and
+    ``commit`` gives back the pages that are out of sight. ``budget``: attention layers see the whole cache, ``commit`` keeps account
+    of the weight each key receives and cuts a sequence that has outgrown ``budget + EVICT_SPARE`` slots back to ``budget``: the
+    first ``sinks`` positions, the ``recent`` latest, and of the others those that received most (``lane_evict``). ``lens`` then counts
+    slots; a sequence's next position in the text is ``position(s)``. With a window, drafted and serial decoding give the same tokens as
+    ever; with a budget what is cut depends on when, and so on how many rows each commit kept."""
 
     def __init__(self, w: Weights, n_seqs: int, max_context: int, device=None, num_pages: int | None = None,
-                 wide: bool = False):
+                 wide: bool = False, window: int | None = None, sinks: int = 0, budget: int | None = None, recent: int = 0):
         c = w.config
         device = device or w.norm.device
+        if window is not None and budget is not None:
+            raise ValueError("State: a window or a budget, not both")
+        if window is not None and window < 1 or sinks < 0 or recent < 0 or (budget is not None and budget < max(1, recent + sinks)):
+            raise ValueError("State: window >= 1 and budget >= recent + sinks required")
+        if window is None and budget is None and (sinks or recent):
+            raise ValueError("State: sinks and recent go with a window or a budget")
+        self.window, self.sinks, self.budget, self.recent = window, sinks, budget, recent
+        if budget is not None:
+            max_context = min(max_context, budget + EVICT_SPARE)
         if wide and w.wide is None:
             raise ValueError("State(wide=True) needs weights prepared by enable_wide")
         self.wide = bool(wide)        # every step of this state multiplies on the wide-row (tcgen05) kernel
@@ -210,12 +227,51 @@ class State:
         self.seq_lens = torch.zeros(n_seqs, dtype=torch.int32, device=device)
         self.gdn_layers = [i for i, l in enumerate(w.layers) if l.linear]
         self.att_layers = [i for i, l in enumerate(w.layers) if not l.linear]
-        pages_per_seq = -(-(max_context + MAX_ROWS) // LA.PAGE)
-        self.kv = LA.PagedKV(len(self.att_layers), n_seqs, num_pages or n_seqs * pages_per_seq, c.kv_heads, c.head_dim,
+        self.dropped = [0] * n_seqs        # positions that eviction has taken out
+        self.max_slots = max_context + MAX_ROWS
+        pages_per_seq = -(-self.max_slots // LA.PAGE)
+        held = pages_per_seq               # at most, by one sequence
+        if window is not None:             # the sinks' pages, the window's with one cut at either end, and those of the rows in flight
+            held = min(held, -(-sinks // LA.PAGE) + -(-(window + MAX_ROWS) // LA.PAGE) + 2)
+        self.kv = LA.PagedKV(len(self.att_layers), n_seqs, num_pages or n_seqs * held, c.kv_heads, c.head_dim,
                              pages_per_seq, device)
         ng = max(len(self.gdn_layers), 1)
         self.conv = torch.zeros((ng, n_seqs, c.conv_kernel - 1, c.conv_channels), dtype=torch.bfloat16, device=device)
         self.rec = torch.zeros((ng, n_seqs, c.v_heads, c.dv, c.dk), dtype=torch.float32, device=device)
+
+        # the size of the key chunks goes into a row's bits: one for all steps of the state
+        self.chunk_keys = lane_window.chunk_keys_for(n_seqs, c.heads, c.kv_heads, 8, self.max_slots, window, sinks) if self.bounded else None
+        self.mass = self.pos = None
+        if budget is not None:
+            self.mass = torch.zeros(self.kv.k.shape[:4], dtype=torch.float32, device=device)
+            self.pos = torch.zeros(self.kv.k.shape[:4], dtype=torch.int32, device=device)
+
+    @property
+    def bounded(self) -> bool:
+        return self.window is not None or self.budget is not None
+
+    def position(self, s: int) -> int:
+        """The position in the text of sequence ``s``'s next token."""
+
+        return self.lens[s] + self.dropped[s]
+
+    def _trim(self) -> None:
+        """Give back what a window has left behind, or cut sequences over their budget back to it."""
+
+        if self.window is not None:
+            for s, n in enumerate(self.lens):
+                self.kv.release_before(s, n, self.window, self.sinks)
+        over = [s for s, n in enumerate(self.lens) if self.budget is not None and n > self.budget + EVICT_SPARE]
+        if over and self.att_layers:
+            dev = self.seq_lens.device
+            lens = torch.tensor([n if s in over else 0 for s, n in enumerate(self.lens)], dtype=torch.int32).to(dev, non_blocking=True)
+            nxt = torch.tensor([self.position(s) for s in range(self.n_seqs)], dtype=torch.int32).to(dev, non_blocking=True)
+            lane_evict.evict(self.kv.k, self.kv.v, self.kv.table, lens, nxt, self.mass, self.pos, self.budget, recent=self.recent, sinks=self.sinks,
+                             max_context=self.max_slots)
+        for s in over:
+            self.dropped[s] += self.lens[s] - self.budget
+            self.lens[s] = self.budget
+            self.kv.shrink(s, self.budget)
 
     def sync_lens(self) -> None:
         self.seq_lens.copy_(torch.tensor(self.lens, dtype=torch.int32), non_blocking=True)
@@ -229,7 +285,10 @@ class State:
 
         from . import build
 
-        return {"kernels": build.source_hash(), "lens": list(self.lens), "rec": self.rec.clone(), "conv": self.conv.clone()}
+        snap = {"kernels": build.source_hash(), "lens": list(self.lens), "rec": self.rec.clone(), "conv": self.conv.clone(), "dropped": list(self.dropped)}
+        if self.budget is not None:
+            snap["mass"], snap["pos"] = self.mass.clone(), self.pos.clone()
+        return snap
 
     def restore(self, snap: dict) -> None:
         from . import build
@@ -240,10 +299,22 @@ class State:
             raise ValueError("State.restore: the snapshot belongs to a differently shaped state")
         if any(self.kv.owned[s] * LA.PAGE < n for s, n in enumerate(snap["lens"])):
             raise ValueError("State.restore: a sequence's pages were released since the snapshot")
+        if self.window is not None and any(self.kv.behind[s] > max(0, n + 1 - self.window) // LA.PAGE for s, n in enumerate(snap["lens"])):
+            raise ValueError("State.restore: pages that the snapshot's window sees were released since")
+        if list(snap.get("dropped", [0] * self.n_seqs)) != self.dropped or (self.budget is not None) != ("mass" in snap):
+            raise ValueError("State.restore: slots were evicted since the snapshot")
+        if self.budget is not None:
+            self.mass.copy_(snap["mass"])
+            self.pos.copy_(snap["pos"])
         self.rec.copy_(snap["rec"])
         self.conv.copy_(snap["conv"])
         self.lens = list(snap["lens"])
         self.sync_lens()
+
+
+# Slots beyond its budget that a sequence may hold before it is cut back (a state with a ``budget``): an eviction ranks all slots, so it
+# is worth doing for a few dozen at a time (16 layers of 4224 slots: 19 us).
+EVICT_SPARE = 128
 
 
 @dataclass
@@ -266,7 +337,7 @@ def _batch_lists(st: State, widths):
     for s, wd in enumerate(widths):
         starts.append(starts[-1] + wd)
         for t in range(wd):
-            seq.append(s); idx.append(t); pos.append(st.lens[s] + t); nk.append(st.lens[s] + t + 1)
+            seq.append(s); idx.append(t); pos.append(st.position(s) + t); nk.append(st.lens[s] + t + 1)
     return starts, seq, idx, pos, nk
 
 
@@ -299,7 +370,8 @@ def make_batch(st: State, widths: Sequence[int], device, max_chunks: int | None 
 @dataclass
 class Record:
     """What a forward leaves for ``commit``: per GDN layer the window's k, v, g, beta and stacked
-    projection rows (qkv for the conv tail), per attention layer the window's K/V rows."""
+    projection rows (qkv for the conv tail), per attention layer the window's K/V rows; where the state has a budget also
+    the attention layers' queries and log-sum-exps."""
 
     batch: Batch
     gdn_k: torch.Tensor
@@ -309,6 +381,8 @@ class Record:
     gdn_in: torch.Tensor
     att_k: torch.Tensor
     att_v: torch.Tensor
+    att_q: torch.Tensor | None = None
+    att_lse: torch.Tensor | None = None
 
 
 @torch.no_grad()
@@ -351,6 +425,9 @@ def tree_forward(w: Weights, tokens: torch.Tensor, windows, st: State, *, full_l
                  torch.empty((ng, R, -(-(2 * kd + 2 * vd + 2 * c.v_heads) // 8) * 8), **bf),
                  torch.empty((na, R, c.kv_heads, c.head_dim), **bf), torch.empty((na, R, c.kv_heads, c.head_dim), **bf))
     q_att = torch.empty((R, c.heads, c.head_dim), **bf)
+    if st.budget is not None:
+        rec.att_q = torch.empty((na, R, c.heads, c.head_dim), **bf)
+        rec.att_lse = torch.empty((na, R, c.heads), dtype=torch.float32, device=dev)
     att_in = torch.empty((R, c.heads * 2 * c.head_dim + 2 * c.kv_heads * c.head_dim), **bf)
     mlp_in = torch.empty((R, 2 * c.intermediate), **bf) if c.experts == 0 else None
     moe_buf = None
@@ -358,7 +435,9 @@ def tree_forward(w: Weights, tokens: torch.Tensor, windows, st: State, *, full_l
         if tp is not None:
             raise ValueError("tree_forward: mixture-of-experts layers shard by expert, not by tensor-parallel rank")
         moe_buf = lane_moe.MoEBuffers(R, c.experts, c.top_k, c.shared_expert, c.hidden, c.moe_intermediate, g, dev)
-    scratch = torch.empty(LA.scratch_bytes(R, c.heads, c.head_dim, b.max_chunks), dtype=torch.uint8, device=dev)
+    need = LA.scratch_bytes(R, c.heads, c.head_dim, b.max_chunks) if not st.bounded else lane_window.scratch_bytes(
+        R, c.heads, c.head_dim, max_window=b.max_window, max_context=st.max_slots, window=st.window, sinks=st.sinks, chunk_keys=st.chunk_keys)
+    scratch = torch.empty(need, dtype=torch.uint8, device=dev)
     scale = c.head_dim ** -0.5
 
     fused_tp = tp is not None and getattr(tp, "fused", False) and not st.wide
@@ -411,13 +490,20 @@ def tree_forward(w: Weights, tokens: torch.Tensor, windows, st: State, *, full_l
             proj = lane_matmul(h, layer.in_proj, out=att_in, next_weight=layer.out_proj)
             nq = c.heads * 2 * c.head_dim
             nkv = c.kv_heads * c.head_dim
+            q = q_att if st.budget is None else rec.att_q[ai]
             lane_glue.attn_prep(proj[:, :nq], proj[:, nq:nq + nkv], proj[:, nq + nkv:], layer.q_norm, layer.k_norm, b.row_pos,
                                 w.inv_freq, c.eps, heads=c.heads, kv_heads=c.kv_heads, head_dim=c.head_dim,
-                                out=(q_att, rec.att_k[ai], rec.att_v[ai]))
+                                out=(q, rec.att_k[ai], rec.att_v[ai]))
             mixed = new_packed(R, c.heads * c.head_dim, g, dev)
-            LA.lane_attention(q_att, rec.att_k[ai], rec.att_v[ai], st.kv.k[ai], st.kv.v[ai], st.kv.table, st.seq_lens,
-                              b.seq_start, b.row_nkeys, scale=scale, max_window=b.max_window, max_chunks=b.max_chunks,
-                              scratch=scratch, gate=proj[:, :nq], packed_out=mixed)      # output gate + packing in the merge
+            if st.bounded:
+                lane_window.window_attention(q, rec.att_k[ai], rec.att_v[ai], st.kv.k[ai], st.kv.v[ai], st.kv.table, st.seq_lens, b.seq_start,
+                                             scale=scale, max_window=b.max_window, max_context=st.max_slots, window=st.window,
+                                             sinks=st.sinks if st.window is not None else 0, chunk_keys=st.chunk_keys, scratch=scratch,
+                                             lse=rec.att_lse[ai] if st.budget is not None else None, gate=proj[:, :nq], packed_out=mixed)
+            else:
+                LA.lane_attention(q, rec.att_k[ai], rec.att_v[ai], st.kv.k[ai], st.kv.v[ai], st.kv.table, st.seq_lens,
+                                  b.seq_start, b.row_nkeys, scale=scale, max_window=b.max_window, max_chunks=b.max_chunks,
+                                  scratch=scratch, gate=proj[:, :nq], packed_out=mixed)  # output gate + packing in the merge
             ai += 1
         r, rparts = row_parallel(mixed, layer.out_proj, layer.gate_up if layer.experts is None else after(li))
         if layer.experts is not None:
@@ -456,8 +542,13 @@ def commit(st: State, record: Record, keep: Sequence[int]) -> None:
         lane_gdn.conv_commit(record.gdn_in, st.conv, b.seq_start, keep_t, st.conv.shape[-1])
     if st.att_layers:
         LA.kv_commit(record.att_k, record.att_v, st.kv, st.seq_lens, b.seq_start, keep_t)
+        if st.budget is not None:
+            lane_evict.attention_mass(record.att_q, record.att_lse, st.kv.k, st.kv.table, st.seq_lens, b.seq_start, keep_t, b.row_pos, st.mass, st.pos,
+                                      scale=st.kv.head_dim ** -0.5, max_window=b.max_window, max_context=st.max_slots)
     for s, k in enumerate(keep):
         st.lens[s] += k
+    if st.bounded:
+        st._trim()
     st.sync_lens()
 
 
@@ -472,5 +563,5 @@ def accept_path(drafted: Sequence[int], verified: Sequence[int]) -> int:
     return n
 
 
-__all__ = ["Batch", "Config", "LayerWeights", "Record", "State", "Weights", "accept_path", "commit", "load_weights",
+__all__ = ["Batch", "Config", "EVICT_SPARE", "LayerWeights", "Record", "State", "Weights", "accept_path", "commit", "load_weights",
            "make_batch", "refresh_batch", "tree_forward"]

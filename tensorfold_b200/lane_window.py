@@ -36,6 +36,14 @@ def chunk_keys_for(n_seqs: int, heads: int, kv_heads: int, max_window: int, max_
     return min(max(-(-keys // 128) * 64, 512), 2048) if columns < 296 else 2048
 
 
+def scratch_bytes(rows: int, heads: int, head_dim: int, *, max_window: int, max_context: int, window: int | None, sinks: int, chunk_keys: int) -> int:
+    """Bytes of ``window_attention``'s scratch."""
+
+    lib = _lib.load()
+    slots = lib.tf_window_slots(0 if window is None else min(window, 1 << 30), sinks if window is not None else 0, max_window, max_context, chunk_keys)
+    return int(lib.tf_window_scratch_bytes(rows, heads, head_dim, slots))
+
+
 def window_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                      page_table: torch.Tensor, seq_lens: torch.Tensor, seq_start: torch.Tensor, *, scale: float, max_window: int,
                      max_context: int, window: int | None = None, sinks: int = 0, chunk_keys: int | None = None,
@@ -70,4 +78,4 @@ def window_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, 
     return packed_out if res is None else res
 
 
-__all__ = ["chunk_keys_for", "window_attention"]
+__all__ = ["chunk_keys_for", "scratch_bytes", "window_attention"]

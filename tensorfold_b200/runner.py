@@ -25,7 +25,8 @@ class LaneRunner:
         self.device = dev
         for s, wd in enumerate(widths):
             if wd:
-                st.kv.reserve(s, max_context + wd)     # pages for the whole run: the captured graph never reallocates
+                # pages for the whole run: the captured graph never reallocates (a bounded state's sequences take theirs step by step)
+                st.kv.reserve(s, st.lens[s] + wd if st.bounded else max_context + wd)
         st.kv.sync_table()
         st.sync_lens()
         from . import lane_attention as LA
@@ -70,6 +71,10 @@ class LaneRunner:
     def refresh(self) -> None:
         """Pick up the state's current lengths (after a commit) for the next replay."""
 
+        if self.st.bounded:                    # pages that a commit gave back may be other sequences' by now
+            taken = [self.st.kv.reserve(s, self.st.lens[s] + wd) for s, wd in enumerate(self.batch.widths) if wd]
+            if any(taken):
+                self.st.kv.sync_table()
         refresh_batch(self.batch, self.st)
         self.st.sync_lens()
         pos = self.batch.row_pos.to(torch.int64) + 1            # the token a row verifies sits one past its input
