@@ -234,12 +234,12 @@ struct Cfg {
     static constexpr int STAGE_ROW = 128 + 16, STAGE_BYTES = kSoftWarps * 32 * STAGE_ROW;      // partials on their way out
     static constexpr int FIT = (227 * 1024 - 2560 - STAGE_BYTES - Q_BYTES) / TILE_BYTES;
     static constexpr int KS = FIT / 2 > 4 ? 4 : FIT / 2, VS = FIT - FIT / 2 > 4 ? 4 : FIT - FIT / 2;
-    static constexpr int NBARS = 2 * KS + 2 * VS + 8 + 2;
+    static constexpr int NBARS = 2 * KS + 2 * VS + 6 + 2;
     static constexpr int SMEM = Q_BYTES + (KS + VS) * TILE_BYTES + STAGE_BYTES + NBARS * 8 + VS * 8 + 1024;
-    // tensor memory: O, two buffers of S, two of P (bf16 pairs)
-    static constexpr int O_COL = 0, S_COL = D, P_COL = D + 2 * kTile, COLS = 512;
+    // tensor memory: O and two buffers of S; P (bf16 pairs) takes the place of the scores it is made from
+    static constexpr int O_COL = 0, S_COL = D, COLS = D == 128 ? 256 : 512;
     static_assert(KS >= 2 && SMEM <= 227 * 1024, "the rings do not fit");
-    static_assert(P_COL + kTile <= COLS, "tensor memory");
+    static_assert(S_COL + 2 * kTile <= COLS, "tensor memory");
     // a block of fewer than 128 rows leaves the last rows of the tensor core's Q operand to whatever follows in shared memory
     static_assert((kRows - QR) * 128 <= (KS + VS) * TILE_BYTES, "the operand's rows lie inside the block's memory");
 };
@@ -270,15 +270,14 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
     auto v_full = [&](int s) { return bars + 8u * (2 * KS + s); };
     auto v_empty = [&](int s) { return bars + 8u * (2 * KS + VS + s); };
     auto s_full = [&](int s) { return bars + 8u * (2 * KS + 2 * VS + s); };
-    auto s_empty = [&](int s) { return bars + 8u * (2 * KS + 2 * VS + 2 + s); };
-    auto p_full = [&](int s) { return bars + 8u * (2 * KS + 2 * VS + 4 + s); };
-    auto o_done = [&](int s) { return bars + 8u * (2 * KS + 2 * VS + 6 + s); };      // P V of a tile is complete
-    const uint32_t q_full = bars + 8u * (2 * KS + 2 * VS + 8), q_empty = q_full + 8;
+    auto p_full = [&](int s) { return bars + 8u * (2 * KS + 2 * VS + 2 + s); };
+    auto o_done = [&](int s) { return bars + 8u * (2 * KS + 2 * VS + 4 + s); };      // P V of a tile is complete
+    const uint32_t q_full = bars + 8u * (2 * KS + 2 * VS + 6), q_empty = q_full + 8;
 
     if (tid == 0) {
         for (int s = 0; s < KS; ++s) { mbar_init(k_full(s), kProducers); mbar_init(k_empty(s), 1); }
         for (int s = 0; s < VS; ++s) { mbar_init(v_full(s), kProducers); mbar_init(v_empty(s), 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(s_full(s), 1); mbar_init(s_empty(s), kSoftWarps); mbar_init(p_full(s), kSoftWarps); mbar_init(o_done(s), 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(s_full(s), 1); mbar_init(p_full(s), kSoftWarps); mbar_init(o_done(s), 1); }
         mbar_init(q_full, 1);
         mbar_init(q_empty, 1);
         mbar_fence_init();
@@ -414,6 +413,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
         }
     } else if (warp == kMmaWarp) {
         // ------------------------------- tensor-core issuer: Q K^T a tile ahead of P V ------------------------------------
+        // The tensor core works in order: scores go where those of the tile before last were once P V, issued before, has read their P; and
+        // that P was there means that they had been read.
         constexpr uint32_t qk_desc = tc_idesc(kTile, false), pv_desc = tc_idesc(D, true);
         const bool leader = elect_one();
         // descriptors as low words that advance by constants; everything the loop depends on is uniform in the compiler's eyes, too: a
@@ -430,7 +431,6 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
             for (int i = 0; i <= tiles; ++i) {
                 if (i < tiles) {
                     const int t = it + i, b = t & 1;
-                    wait(s_empty(b), (uint32_t)(((t >> 1) & 1) ^ 1));
                     wait(k_full(kr.i), kr.phase);
                     tc_fence_after();
                     const uint32_t k_lo = desc_lo(smem_u32(k_s) + kr.i * C::TILE_BYTES, 1), d = tmem + C::S_COL + b * kTile;
@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
                     const uint32_t v_lo = desc_lo(smem_u32(v_s) + vr.i * C::TILE_BYTES, kPage * 128 / 16);
 #pragma unroll
                     for (int pg = 0; pg < kTile / kPage; ++pg)
-                        tc_mma_ts(leader, tmem + C::O_COL, tmem + C::P_COL + b * (kTile / 2) + pg * 8, v_lo + pg * (C::PAGE_BYTES >> 4), pv_desc, i > 1 || pg > 0);
+                        tc_mma_ts(leader, tmem + C::O_COL, tmem + C::S_COL + b * kTile + pg * 8, v_lo + pg * (C::PAGE_BYTES >> 4), pv_desc, i > 1 || pg > 0);
                     if (leader) { tc_commit(o_done(b)); tc_commit(v_empty(vr.i)); }
                     vr.next();
                     __syncwarp();
@@ -474,8 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
             if (warp * 32 >= w.nq) {                     // no rows: keeps step with the others, tile by tile
                 for (int i = 0; i < w.tiles; ++i, ++it, vr.next()) {
                     wait(s_full(it & 1), (uint32_t)((it >> 1) & 1));
-                    if (it > 1) wait(o_done(it & 1), (uint32_t)((it >> 1) & 1) ^ 1u);
-                    if (lane == 0) { mbar_arrive(s_empty(it & 1)); mbar_arrive(p_full(it & 1)); }
+                    if (lane == 0) mbar_arrive(p_full(it & 1));
                 }
                 continue;
             }
@@ -494,9 +493,6 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
                 tc_ld32(row + C::S_COL + b * kTile, *reinterpret_cast<float(*)[32]>(s));
                 tc_ld32(row + C::S_COL + b * kTile + 32, *reinterpret_cast<float(*)[32]>(s + 32));
                 tc_wait_ld();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(s_empty(b));
                 if (!plain) {                            // the V tile's notes are there once it is (and stay until P V)
                     uint32_t bad[2] = {0, 0};
                     if (w.p_first != w.p_last) {         // (a row alone sees all that is read)
@@ -561,9 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
                 float s0, s1;
                 split_pair(add_pair(add_pair(sum[0], sum[1]), add_pair(sum[2], sum[3])), s0, s1);
                 l += s0 + s1;
-                if (it > 1) wait(o_done(b), round ^ 1u);             // P V of the tile before last has read this buffer
-                tc_fence_after();
-                tc_st32(row + C::P_COL + b * (kTile / 2), pk);
+                tc_st32(row + C::S_COL + b * kTile, pk);
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
