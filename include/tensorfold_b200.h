@@ -313,8 +313,8 @@ int tf_lane_attention_paged_static(const void* q, const void* k_new, const void*
  * (sinks then change nothing). Keys are cut by absolute position into chunks of chunk_keys (a multiple of 64) that are
  * attended by themselves and joined in order, so a row's bits depend on chunk_keys and on its own keys only. A call's partials
  * live in `slots` = tf_window_slots(...) chunks of scratch (tf_window_scratch_bytes, 16-byte aligned, no initialisation; calls that overlap
- * on the GPU must not share it). tf_window_launches: how many kernels a call queues: the chunks and the join, before them a plan where
- * blocks take several chunks. q, k_new, v_new, pages, out 16-byte aligned. num_pages bounds the page numbers: an entry
+ * on the GPU must not share it). tf_window_launches: how many kernels a call queues: the chunks, before them a plan where blocks take
+ * several of them, behind them a join unless there is one slot and the call is plain (neither qg nor out_packed). q, k_new, v_new, pages, out 16-byte aligned. num_pages bounds the page numbers: an entry
  * outside [0, num_pages) on a page that a row sees is reported as TF_EINVAL through `status` and its keys are left out; entries of
  * pages that no row sees are not read. max_window bounds a sequence's rows, max_context its keys with its window's own (also
  * reported). lse, when not NULL, receives ln(sum exp(score)) [rows, heads] fp32. Rows behind seq_start[n_seqs] are left as
@@ -322,7 +322,7 @@ int tf_lane_attention_paged_static(const void* q, const void* k_new, const void*
  * rows of a page, later rows) may hold anything; a row that sees a value that is not finite has no specified result. */
 int tf_window_slots(int window, int sinks, int max_window, int max_context, int chunk_keys);
 size_t tf_window_scratch_bytes(int rows, int heads, int head_dim, int slots);
-int tf_window_launches(int rows, int n_seqs, int max_window, int slots, int heads, int kv_heads);
+int tf_window_launches(int rows, int n_seqs, int max_window, int slots, int heads, int kv_heads, int head_dim, int plain);
 int tf_window_attention(const void* q, const void* k_new, const void* v_new, const void* k_pages, const void* v_pages, int num_pages,
                         const int* page_table, int max_pages, const int* seq_lens, const int* seq_start, void* out, float* lse,
                         const void* qg, size_t qg_stride, void* out_packed, int group, void* scratch, size_t scratch_bytes, int rows,

@@ -351,7 +351,7 @@ PyObject* window_attention_py(PyObject* const* args, Py_ssize_t n) {
                                    (int)d, (float)scale, status, stream.stream());
     }();
     check_rc(rc, "window_attention");
-    g_launches.fetch_add(tf_window_launches((int)r, (int)s, max_window, slots, (int)h, (int)hk), std::memory_order_relaxed);
+    g_launches.fetch_add(tf_window_launches((int)r, (int)s, max_window, slots, (int)h, (int)hk, (int)d, !gate.defined() && !packed.defined()), std::memory_order_relaxed);
     if (!out.defined()) Py_RETURN_NONE;
     return THPVariable_Wrap(out);
 }

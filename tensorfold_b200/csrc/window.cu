@@ -56,8 +56,9 @@ struct WindowArgs {
     int chunk, first_slots, near_slots, slots;         // keys a chunk; slots of the sinks' chunks, of the window's, of both
     int qgroups, group_rows, items;                    // groups of window rows, rows a group; (group, slot, KV head, sequence) in all
     FastDiv by_group, by_slot, by_head, by_G, by_chunk;
-    int* plan;                         // [rounds, kSms] items by block, -1: none; null: block b takes items b, b + blocks, ...
-    int rounds;
+    int* plan;                         // [rounds, blocks] items by block, -1: none; null: block b takes items b, b + blocks, ...
+    int rounds, blocks;                // blocks: of a full GPU
+    bool direct;                       // one chunk a row and nothing to be done to the results: no join
     float scale_log2;
 };
 
@@ -162,7 +163,7 @@ struct Walk {
     Raw raw;
     __device__ explicit Walk(const WindowArgs& a) : item(at(a, 0)), next(at(a, 1)), raw(fetch(a, item)) {}
     __device__ static int at(const WindowArgs& a, int k) {
-        if (a.plan != nullptr) return k < a.rounds ? a.plan[k * kSms + blockIdx.x] : -1;
+        if (a.plan != nullptr) return k < a.rounds ? a.plan[k * a.blocks + blockIdx.x] : -1;
         const int i = blockIdx.x + k * gridDim.x;
         return i < a.items ? i : -1;
     }
@@ -181,14 +182,14 @@ struct Walk {
 // the blocks end together (16 users: 40 tiles of 64 keys on the busiest block without it, 28 on average). One block; the
 // order among equals does not matter, no item's result depends on where it runs.
 constexpr int kPlanThreads = 1024, kPlanItems = 8192, kPlanBins = 128;
-constexpr size_t kPlanBytes = ((kPlanItems + kSms - 1) / kSms * kSms * sizeof(int) + 255) / 256 * 256;
+constexpr size_t kPlanBytes = ((kPlanItems + 2 * kSms) * sizeof(int) + 255) / 256 * 256;
 __global__ void __launch_bounds__(kPlanThreads) window_plan_kernel(const WindowArgs a) {
     __shared__ int count[kPlanBins], start[kPlanBins];
     pdl_launch_dependents();
     const int tid = threadIdx.x;
     if (tid < kPlanBins) count[tid] = 0;
     pdl_wait();                                  // the plan may still be the one of a call before this
-    for (int i = tid; i < a.rounds * kSms; i += kPlanThreads) a.plan[i] = -1;
+    for (int i = tid; i < a.rounds * a.blocks; i += kPlanThreads) a.plan[i] = -1;
     __syncthreads();
     constexpr int PER = kPlanItems / kPlanThreads;
     int place[PER];                              // bin << 16 | rank in it
@@ -221,24 +222,30 @@ __global__ void __launch_bounds__(kPlanThreads) window_plan_kernel(const WindowA
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
         if (place[k] < 0) continue;
-        const int at = start[place[k] >> 16] + (place[k] & 0xFFFF), round = at / kSms, in_round = at - round * kSms;
-        a.plan[round * kSms + (round & 1 ? kSms - 1 - in_round : in_round)] = tid + k * kPlanThreads;
+        const int at = start[place[k] >> 16] + (place[k] & 0xFFFF), round = at / a.blocks, in_round = at - round * a.blocks;
+        a.plan[round * a.blocks + (round & 1 ? a.blocks - 1 - in_round : in_round)] = tid + k * kPlanThreads;
     }
 }
+
+// Blocks an SM: with heads of 128 a second one fits, and one's softmax runs beside the other's products; heads of 256 fill the
+// shared memory.
+__host__ __device__ constexpr int blocks_of(int head_dim) { return head_dim == 128 ? 2 : 1; }
 
 template <int D, int QR>
 struct Cfg {
     static constexpr int SLABS = D / 64;                 // 64 values of a row: one 128-byte swizzle row
     static constexpr int Q_SLAB = QR * 128, Q_BYTES = SLABS * Q_SLAB;
     static constexpr int TILE_BYTES = kTile * D * 2, K_SLAB = kTile * 128, PAGE_BYTES = kPage * D * 2;
-    static constexpr int STAGE_ROW = 128 + 16, STAGE_BYTES = kSoftWarps * 32 * STAGE_ROW;      // partials on their way out
-    static constexpr int FIT = (227 * 1024 - 2560 - STAGE_BYTES - Q_BYTES) / TILE_BYTES;
+    static constexpr int BLOCKS = blocks_of(D), MEMORY = (BLOCKS == 2 ? 113 : 227) * 1024;
+    // results on their way out: 16 or 32 partial values a row, or 32 finished ones
+    static constexpr int STAGE = BLOCKS == 2 ? 16 : 32, STAGE_ROW = STAGE * 4 + 16, STAGE_BYTES = kSoftWarps * 32 * STAGE_ROW;
+    static constexpr int FIT = (MEMORY - 2560 - STAGE_BYTES - Q_BYTES) / TILE_BYTES;
     static constexpr int KS = FIT / 2 > 4 ? 4 : FIT / 2, VS = FIT - FIT / 2 > 4 ? 4 : FIT - FIT / 2;
     static constexpr int NBARS = 2 * KS + 2 * VS + 6 + 2;
     static constexpr int SMEM = Q_BYTES + (KS + VS) * TILE_BYTES + STAGE_BYTES + NBARS * 8 + VS * 8 + 1024;
     // tensor memory: O and two buffers of S; P (bf16 pairs) takes the place of the scores it is made from
     static constexpr int O_COL = 0, S_COL = D, COLS = D == 128 ? 256 : 512;
-    static_assert(KS >= 2 && SMEM <= 227 * 1024, "the rings do not fit");
+    static_assert(KS >= 2 && SMEM + 64 <= MEMORY, "the rings do not fit");
     static_assert(S_COL + 2 * kTile <= COLS, "tensor memory");
     // a block of fewer than 128 rows leaves the last rows of the tensor core's Q operand to whatever follows in shared memory
     static_assert((kRows - QR) * 128 <= (KS + VS) * TILE_BYTES, "the operand's rows lie inside the block's memory");
@@ -251,7 +258,7 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
 }
 
 template <int D, int QR>
-__global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_constant__ WindowArgs a, const __grid_constant__ CUtensorMap q_map,
+__global__ void __launch_bounds__(kThreads, blocks_of(D)) window_chunk_kernel(const __grid_constant__ WindowArgs a, const __grid_constant__ CUtensorMap q_map,
                                                                    const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                                                                    const __grid_constant__ CUtensorMap kn_map, const __grid_constant__ CUtensorMap vn_map) {
     using C = Cfg<D, QR>;
@@ -489,10 +496,9 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
                 const bool plain = w.plain(j0);
                 wait(s_full(b), round);
                 tc_fence_after();
-                float s[kTile];
-                tc_ld32(row + C::S_COL + b * kTile, *reinterpret_cast<float(*)[32]>(s));
-                tc_ld32(row + C::S_COL + b * kTile + 32, *reinterpret_cast<float(*)[32]>(s + 32));
-                tc_wait_ld();
+                // a part of the scores at a time, read twice where there are two (two blocks an SM have 96 registers a thread)
+                constexpr int PART = C::BLOCKS == 2 ? kTile / 2 : kTile;
+                uint32_t see[2] = {~0u, ~0u};            // bit e: the row sees key j0 + e; up to p, and from lo on or below the sinks' end
                 if (!plain) {                            // the V tile's notes are there once it is (and stay until P V)
                     uint32_t bad[2] = {0, 0};
                     if (w.p_first != w.p_last) {         // (a row alone sees all that is read)
@@ -500,23 +506,32 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
                         bad[0] = bad_s[vr.i * 2];
                         bad[1] = bad_s[vr.i * 2 + 1];
                     }
-                    // bit e: the row sees key j0 + e; up to p, and from lo on or below the sinks' end
                     auto below = [](int x) -> unsigned long long { return x <= 0 ? 0ull : x >= kTile ? ~0ull : (1ull << x) - 1; };
                     const unsigned long long sees = below(p + 1 - j0) & (~below(lo - j0) | below(w.sinks - j0));
-                    const uint32_t see[2] = {(uint32_t)sees, (uint32_t)(sees >> 32)};
+                    see[0] = (uint32_t)sees;
+                    see[1] = (uint32_t)(sees >> 32);
                     if ((see[0] & bad[0]) | (see[1] & bad[1])) l = __int_as_float(0x7FC00000);
-#pragma unroll
-                    for (int e = 0; e < kTile; ++e) s[e] = see[e >> 5] >> (e & 31) & 1 ? s[e] : -INFINITY;
                 }
                 vr.next();
-                float tops[4];
+                float s[PART];
+                auto scores = [&](int e0) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) tops[e] = s[e];
+                    for (int c = 0; c < PART; c += 32) tc_ld32(row + C::S_COL + b * kTile + e0 + c, *reinterpret_cast<float(*)[32]>(s + c));
+                    tc_wait_ld();
+                    if (!plain) {
 #pragma unroll
-                for (int e = 4; e + 7 < kTile + 4; e += 8) {
+                        for (int e = 0; e < PART; ++e) s[e] = see[PART == kTile ? e >> 5 : e0 >> 5] >> (e & 31) & 1 ? s[e] : -INFINITY;
+                    }
+                };
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (e + 2 * k + 1 < kTile) tops[k] = max3(tops[k], s[e + 2 * k], s[e + 2 * k + 1]);
+                for (int e0 = 0; e0 < kTile; e0 += PART) {
+                    scores(e0);
+#pragma unroll
+                    for (int e = 0; e < PART; e += 8) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) tops[k] = max3(tops[k], s[e + 2 * k], s[e + 2 * k + 1]);
+                    }
                 }
                 const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * a.scale_log2;
                 // move the maximum only where it must: a row's choice looks at its own scores alone
@@ -543,54 +558,83 @@ __global__ void __launch_bounds__(kThreads, 1) window_chunk_kernel(const __grid_
                 const float off = m == -INFINITY ? 0.f : -m;
                 const unsigned long long off2 = pair_of(off, off);
                 unsigned long long sum[4] = {0, 0, 0, 0};            // two zeros each
-                uint32_t pk[kTile / 2];
 #pragma unroll
-                for (int e = 0; e < kTile; e += 2) {
-                    float x, y;
-                    split_pair(fma_pair(pair_of(s[e], s[e + 1]), scale2, off2), x, y);
-                    x = fast_exp2(x);
-                    y = fast_exp2(y);
-                    sum[(e >> 1) & 3] = add_pair(sum[(e >> 1) & 3], pair_of(x, y));
-                    const __nv_bfloat162 xy = __floats2bfloat162_rn(x, y);
-                    pk[e >> 1] = *reinterpret_cast<const uint32_t*>(&xy);
+                for (int e0 = 0; e0 < kTile; e0 += PART) {
+                    if (PART < kTile) scores(e0);
+                    uint32_t pk[PART / 2];
+#pragma unroll
+                    for (int e = 0; e < PART; e += 2) {
+                        float x, y;
+                        split_pair(fma_pair(pair_of(s[e], s[e + 1]), scale2, off2), x, y);
+                        x = fast_exp2(x);
+                        y = fast_exp2(y);
+                        sum[(e >> 1) & 3] = add_pair(sum[(e >> 1) & 3], pair_of(x, y));
+                        const __nv_bfloat162 xy = __floats2bfloat162_rn(x, y);
+                        pk[e >> 1] = *reinterpret_cast<const uint32_t*>(&xy);
+                    }
+                    if constexpr (PART == kTile) tc_st32(row + C::S_COL + b * kTile, pk);
+                    else tc_st16(row + C::S_COL + b * kTile + e0 / 2, pk);
                 }
                 float s0, s1;
                 split_pair(add_pair(add_pair(sum[0], sum[1]), add_pair(sum[2], sum[3])), s0, s1);
                 l += s0 + s1;
-                tc_st32(row + C::S_COL + b * kTile, pk);
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full(b));
             }
-            // ---- the chunk's partials ----
-            const size_t first = (size_t)w.slot * a.R * a.H;
-            if (mine) { a.part_m[first + q_row] = m; a.part_l[first + q_row] = l; }
-            // 32 values of 32 rows at a time through shared memory, so that a store covers whole lines; a lane's rows are 4 x + lane / 8
+            // ---- the chunk's partials, or the results where a row has one chunk: 32 columns at a time through shared memory, so that a
+            // store covers whole sectors ----
             const int rows_here = min(32, w.nq - warp * 32);
-            float* to[8];
+            constexpr int LANES = C::STAGE / 4, ROWS = 32 / LANES;       // lanes a row of partials, rows a store
+            const size_t first = (size_t)w.slot * a.R * a.H;
+            float* to[LANES];
+            float inv = 0.f;
+            if (a.direct) {
+                inv = 1.f / l;
+                if (mine && a.lse != nullptr) a.lse[q_row] = (m + log2f(l)) * kLn2;
+            } else {
+                if (mine) { a.part_m[first + q_row] = m; a.part_l[first + q_row] = l; }
 #pragma unroll
-            for (int x = 0; x < 8; ++x) to[x] = a.part_o + (first + __shfl_sync(0xffffffffu, q_row, x * 4 + (lane >> 3))) * D + (lane & 7) * 4;
+                for (int x = 0; x < LANES; ++x) to[x] = a.part_o + (first + __shfl_sync(0xffffffffu, q_row, x * ROWS + lane / LANES)) * D + lane % LANES * 4;
+            }
             wait(o_done((it - 1) & 1), (uint32_t)(((it - 1) >> 1) & 1));
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < D; c += 64) {
-                float o[2][32];
-                tc_ld32(row + C::O_COL + c, o[0]);
-                tc_ld32(row + C::O_COL + c + 32, o[1]);
+            for (int c = 0; c < D; c += 32) {
+                float o[32];
+                tc_ld32(row + C::O_COL + c, o);
                 tc_wait_ld();
+                uint8_t* const cell = mine_s + lane * C::STAGE_ROW;
+                if (a.direct) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                    for (int e = 0; e < 32; e += 8) {
+                        float x[8];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4)
-                        *reinterpret_cast<float4*>(mine_s + lane * C::STAGE_ROW + e * 4) = make_float4(o[h][e], o[h][e + 1], o[h][e + 2], o[h][e + 3]);
+                        for (int y = 0; y < 8; ++y) x[y] = o[e + y] * inv;
+                        *reinterpret_cast<uint4*>(cell + e * 2) = pack8(x);
+                    }
                     __syncwarp();
-                    float4 v[8];
 #pragma unroll
-                    for (int x = 0; x < 8; ++x) v[x] = *reinterpret_cast<const float4*>(mine_s + (x * 4 + (lane >> 3)) * C::STAGE_ROW + (lane & 7) * 16);
+                    for (int x = 0; x < 4; ++x) {
+                        const int r = x * 8 + (lane >> 2), at = __shfl_sync(0xffffffffu, q_row, r);
+                        const uint4 v = *reinterpret_cast<const uint4*>(mine_s + r * C::STAGE_ROW + (lane & 3) * 16);
+                        if (r < rows_here) *reinterpret_cast<uint4*>(a.out + (size_t)at * D + c + (lane & 3) * 8) = v;
+                    }
+                    __syncwarp();
+                    continue;
+                }
 #pragma unroll
-                    for (int x = 0; x < 8; ++x)
-                        if (x * 4 + (lane >> 3) < rows_here) *reinterpret_cast<float4*>(to[x] + c + h * 32) = v[x];
+                for (int h = 0; h < 32; h += C::STAGE) {
+#pragma unroll
+                    for (int e = 0; e < C::STAGE; e += 4) *reinterpret_cast<float4*>(cell + e * 4) = make_float4(o[h + e], o[h + e + 1], o[h + e + 2], o[h + e + 3]);
+                    __syncwarp();
+                    float4 v[LANES];
+#pragma unroll
+                    for (int x = 0; x < LANES; ++x) v[x] = *reinterpret_cast<const float4*>(mine_s + (x * ROWS + lane / LANES) * C::STAGE_ROW + lane % LANES * 16);
+#pragma unroll
+                    for (int x = 0; x < LANES; ++x)
+                        if (x * ROWS + lane / LANES < rows_here) *reinterpret_cast<float4*>(to[x] + c + h) = v[x];
                     __syncwarp();
                 }
             }
@@ -663,9 +707,10 @@ __global__ void __launch_bounds__(128) window_join_kernel(const WindowArgs a) {
         }
     }
     if (a.lse != nullptr && li == 0 && there) a.lse[(size_t)row * a.H + head] = (m + log2f(l)) * kLn2;
+    const float inv = 1.f / l;               // (one chunk: the same operations as where the chunk kernel writes the results)
     float o[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = round_bf16(acc[e] / l);
+    for (int e = 0; e < 8; ++e) o[e] = round_bf16(acc[e] * inv);
     if (a.qg != nullptr && there) {
         float g[8];
         unpack8(*reinterpret_cast<const uint4*>(a.qg + (size_t)row * a.qg_stride + (size_t)head * 2 * D + D + li * 8), g);
@@ -707,7 +752,7 @@ int launch_chunks(const WindowArgs& a, cudaStream_t st) {
         !describe_rows(&maps[4], a.v_new, D, R < 16 ? 16 : R, row * HK, HK, row, false, kPage, 1, D / 64))
         return TF_ECUDA;
     void* args[] = {const_cast<WindowArgs*>(&a), &maps[0], &maps[1], &maps[2], &maps[3], &maps[4]};
-    if (launch_pdl((const void*)window_chunk_kernel<D, QR>, dim3(a.items < kSms ? a.items : kSms), dim3(kThreads), C::SMEM, st, args) != cudaSuccess) {
+    if (launch_pdl((const void*)window_chunk_kernel<D, QR>, dim3(a.items < a.blocks ? a.items : a.blocks), dim3(kThreads), C::SMEM, st, args) != cudaSuccess) {
         cudaGetLastError();
         return TF_ECUDA;
     }
@@ -725,21 +770,22 @@ bool cut_rows(WindowArgs& a) {
     return items <= (1 << 30);
 }
 // A plan only where a block takes several items, and not so many that they even out.
-bool planned(int items) { return items > kSms && items <= kPlanItems; }
+bool planned(const WindowArgs& a) { return a.items > a.blocks && a.items <= kPlanItems; }
 
 template <int D>
 int run(WindowArgs& a, cudaStream_t st) {
     const int G = a.H / a.HK;
     if (!cut_rows(a)) return TF_EINVAL;
     a.by_group = fast_div(a.qgroups); a.by_slot = fast_div(a.slots); a.by_head = fast_div(a.HK); a.by_G = fast_div(G); a.by_chunk = fast_div(a.chunk);
-    a.rounds = (a.items + kSms - 1) / kSms;
-    if (!planned(a.items)) a.plan = nullptr;
+    a.blocks = kSms * blocks_of(D);
+    a.rounds = (a.items + a.blocks - 1) / a.blocks;
+    if (!planned(a)) a.plan = nullptr;
     if (a.plan != nullptr) {
         void* args[] = {&a};
         if (launch_pdl((const void*)window_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, args) != cudaSuccess) { cudaGetLastError(); return TF_ECUDA; }
     }
     const int rc = a.group_rows * G <= 64 ? launch_chunks<D, 64>(a, st) : launch_chunks<D, 128>(a, st);
-    if (rc != TF_OK) return rc;
+    if (rc != TF_OK || a.direct) return rc;
     void* join[] = {&a};
     const int heads = 4 * (32 / (D / 8)), out_rows = a.out_packed ? tf_padded_rows(a.R) : a.R;
     // (one row of 7 chunks: 11.3 us with eight in flight, 12 with four; 2900 rows of one or two: 14 and 24 us for this kernel)
@@ -768,11 +814,12 @@ size_t tf_window_scratch_bytes(int rows, int heads, int head_dim, int slots) {
     return tf::kPlanBytes + (size_t)slots * rows * heads * (head_dim + 2) * sizeof(float);
 }
 
-int tf_window_launches(int rows, int n_seqs, int max_window, int slots, int heads, int kv_heads) {
+int tf_window_launches(int rows, int n_seqs, int max_window, int slots, int heads, int kv_heads, int head_dim, int plain) {
     if (rows < 1 || n_seqs < 1 || max_window < 1 || slots < 1 || kv_heads < 1 || heads < kv_heads || heads / kv_heads > 16) return 0;
     tf::WindowArgs a{};
     a.R = rows; a.S = n_seqs; a.max_window = max_window; a.slots = slots; a.H = heads; a.HK = kv_heads;
-    return !tf::cut_rows(a) ? 0 : tf::planned(a.items) ? 3 : 2;
+    a.blocks = tf::kSms * tf::blocks_of(head_dim);
+    return !tf::cut_rows(a) ? 0 : 1 + (tf::planned(a) ? 1 : 0) + (slots == 1 && plain ? 0 : 1);
 }
 
 int tf_window_attention(const void* q, const void* k_new, const void* v_new, const void* k_pages, const void* v_pages, int num_pages,
@@ -804,6 +851,7 @@ int tf_window_attention(const void* q, const void* k_new, const void* v_new, con
     a.scale_log2 = scale * tf::kLog2e;
     a.max_window = max_window;
     a.chunk = chunk_keys; a.slots = slots;
+    a.direct = slots == 1 && !qg && !out_packed;
     const tf::Slots cut = tf::slots_for(window, sinks, max_window, max_context, chunk_keys);
     a.first_slots = cut.first; a.near_slots = cut.near > 0 ? cut.near : 1;
     const size_t cells = (size_t)slots * rows * heads;

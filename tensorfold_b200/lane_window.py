@@ -20,9 +20,12 @@ def chunk_keys_for(n_seqs: int, heads: int, kv_heads: int, max_window: int, max_
     pieces that are attended by themselves and joined.
 
     Few columns (sequence, KV head, group of up to 128 query rows): as many chunks as leave the SMs one each, but not below the size at
-    which a chunk's tiles (0.95 us for 64 keys) and the join (0.36 us a chunk) cost the same. More: half of what a
-    group sees, so that the chunks can be dealt out evenly (16 x 4 columns of 4100 keys: 61 us in chunks of 2048, 68 of 512, 78 of
-    4096); very many, as for a prompt's rows: 2048 (500 columns of 1040 keys: 68 us, 77 of 512).
+    which a chunk's tiles (0.95 us for 64 keys) and the join (0.36 us a chunk) cost the same, and one chunk where that saves
+    the join for few tiles more (300 rows of up to 400 keys: 16.8 us in one, 21.1 in two). More columns: a quarter of what a group sees, so that the
+    chunks can be dealt out evenly (16 x 4 columns of 4100 keys: 59.1 us in chunks of 1024, 59.6 of 2048, 64.8 of 512, 77 of 4096; with heads
+    of 128 38.7, 48.7, 43.3 and 71.6). Very many, as for a prompt's rows: one chunk, without partials and join, where a group sees few
+    keys (362 columns of 1040 keys: 45.5 us, 57 in chunks of 2048; 576 of 4000: 222 and 284), else 2048 (376 columns of 17500
+    keys: 511 us, 643 in one chunk, whose columns do not divide evenly).
     """
 
     if min(n_seqs, kv_heads, max_window) < 1 or heads < kv_heads or max_context < max_window:
@@ -30,10 +33,14 @@ def chunk_keys_for(n_seqs: int, heads: int, kv_heads: int, max_window: int, max_
     rows = max(1, min(max_window, 128 // (heads // kv_heads)))
     columns = n_seqs * kv_heads * -(-max_window // rows)
     keys = max_context if window is None else min(max_context, window + rows - 1)
+    whole = -(-max(max_context, 128) // 64) * 64
     spare = 148 // columns - (0 if window is None else 1 + (sinks > 0))       # a window lies across one chunk more, sinks have their own
     if spare >= 1:
-        return -(-max(128, math.isqrt(24 * keys), -(-keys // spare)) // 64) * 64
-    return min(max(-(-keys // 128) * 64, 512), 2048) if columns < 296 else 2048
+        chunk = -(-max(128, math.isqrt(24 * keys), -(-keys // spare)) // 64) * 64
+        return whole if whole - chunk <= 256 else chunk
+    if columns < 222:
+        return min(max(-(-keys // 256) * 64, 512), 2048)
+    return whole if keys <= 4096 else 2048
 
 
 def scratch_bytes(rows: int, heads: int, head_dim: int, *, max_window: int, max_context: int, window: int | None, sinks: int, chunk_keys: int) -> int:

@@ -78,12 +78,14 @@ def test_slots_cover_any_window(lib):
 
 
 def test_launch_counts(lib):
-    assert lib.tf_window_launches(1, 1, 1, 32, 24, 4) == 2                 # 128 items: a block each
-    assert lib.tf_window_launches(1, 1, 1, 38, 24, 4) == 3                 # 152: some blocks take two
-    assert lib.tf_window_launches(128, 16, 8, 128, 24, 4) == 3             # 8192
-    assert lib.tf_window_launches(128, 16, 8, 129, 24, 4) == 2
-    assert lib.tf_window_launches(128, 16, 100, 20, 24, 4) == 3            # 5 groups of 21 rows
-    assert lib.tf_window_launches(0, 1, 1, 1, 1, 1) == lib.tf_window_launches(1, 1, 1, 1, 34, 2) == lib.tf_window_launches(1, 1 << 15, 1, 1 << 15, 4, 4) == 0
+    assert lib.tf_window_launches(1, 1, 1, 32, 24, 4, 256, 1) == 2                 # 128 items: a block each
+    assert lib.tf_window_launches(1, 1, 1, 38, 24, 4, 256, 1) == 3                 # 152: some blocks take two
+    assert lib.tf_window_launches(128, 16, 8, 128, 24, 4, 256, 1) == 3             # 8192
+    assert lib.tf_window_launches(128, 16, 8, 129, 24, 4, 256, 1) == 2
+    assert lib.tf_window_launches(128, 16, 100, 20, 24, 4, 256, 1) == 3            # 5 groups of 21 rows
+    assert [lib.tf_window_launches(1, seqs, 1, 1, 24, 4, 256, plain) for seqs, plain in ((2, 1), (2, 0), (60, 1), (60, 0))] == [1, 2, 2, 3]
+    assert lib.tf_window_launches(0, 1, 1, 1, 1, 1, 128, 1) == lib.tf_window_launches(1, 1, 1, 1, 34, 2, 128, 1) == lib.tf_window_launches(1, 1 << 15, 1, 1 << 15, 4, 4, 128, 1) == 0
+    assert lib.tf_window_launches(1, 1, 1, 74, 24, 4, 128, 1) == 2 and lib.tf_window_launches(1, 1, 1, 75, 24, 4, 128, 1) == 3      # two blocks an SM
 
 
 def test_refusals_before_any_launch(lib):

@@ -126,6 +126,21 @@ def test_other_chunks(lib, chunk):
 
 @pytest.mark.parametrize("h,hk,d", [(24, 4, 256), (16, 2, 128)])
 @pytest.mark.parametrize("window,sinks", [(None, 0), (130, 4), (64, 20)])
+def test_a_chunk_a_row_gives_the_bits_of_the_join(lib, h, hk, d, window, sinks):
+    """max_context decides whether there is one slot, and with it the way the results take."""
+
+    lens, widths = [400, 3, 0, 77, 511], [9, 140, 1, 0, 1]
+    c = make(41, lens, widths, h, hk, d, extra_rows=2)
+    one, lse = attend(c, lens, widths, window, sinks, chunk=512, context=512)
+    two, lse2 = attend(c, lens, widths, window, sinks, chunk=512, context=513)
+    assert_same_bits(one, two)
+    assert_same_bits(lse, lse2)
+    assert bool((one[-2:] == 55).all()) and bool((lse[-2:] == 77).all())
+    check(c, one, lse, lens, widths, window, sinks)
+
+
+@pytest.mark.parametrize("h,hk,d", [(24, 4, 256), (16, 2, 128)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (130, 4), (64, 20)])
 def test_a_window_has_the_bits_of_serial_steps(lib, h, hk, d, window, sinks):
     lens, widths = [500, 121, 9], [8, 7, 8]
     c = make(7, lens, widths, h, hk, d)
