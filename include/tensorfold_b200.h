@@ -485,7 +485,7 @@ int tf_sample_rows(const int* idx, const float* val, int width, const long long*
  * row t + 1 / draft_temperature), or all of q on the draft itself where draft_logits is NULL, row t + 1 is kept while
  * uniforms[t][0] * q(draft) < p(draft); keep[s] counts the kept rows with row 0. next[s] is the first token in vocabulary order
  * whose cumulative weight is above uniforms[t][1] times the total, t the last kept row: the weights are max(p - q, 0) where row t + 1 was
- * refused (p itself if that leaves nothing), and p where the window was kept whole. A sequence without rows gives keep 0 and next -1, a
+ * refused (p itself if that leaves nothing), and p where the window was kept whole. A sequence without rows, or with rows outside the call's, gives keep 0 and next -1, a
  * row without any probability (every logit -inf or NaN) keeps no draft and gives next -1; logits above 7e8
  * temperatures, +inf among them, count as that many; a draft outside the vocabulary is refused. uniforms [rows, 2] in [0, 1), fp32 or (uniforms_f64) fp64. logits, draft_logits:
  * rows of vocab bf16, any alignment, row strides in elements. scratch: tf_verify_scratch_bytes, 8-byte aligned, no initialisation; two launches.

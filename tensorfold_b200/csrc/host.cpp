@@ -296,7 +296,11 @@ template <class T>
 T* data_of(const at::Tensor& t) { return t.defined() ? static_cast<T*>(t.mutable_data_ptr()) : nullptr; }
 // The caller's buffer or one of `bytes` from the allocator. (A buffer that is too small is refused by the entry point.)
 at::Tensor buffer(PyObject* given, size_t bytes, const at::Tensor& like) {
-    if (given != Py_None) return tensor(given);
+    if (given != Py_None) {
+        at::Tensor t = tensor(given);
+        need(t.is_contiguous(), "scratch must be contiguous");
+        return t;
+    }
     return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
 }
 size_t bytes_of(const at::Tensor& t) { return (size_t)t.numel() * t.element_size(); }
@@ -324,7 +328,7 @@ PyObject* window_attention_py(PyObject* const* args, Py_ssize_t n) {
     const int64_t r = q.size(0), h = q.size(1), d = q.size(2), hk = k_new.size(1), s = lens.size(0);
     need(r >= 1 && s >= 1 && h >= 1 && hk >= 1 && k_new.size(0) == r && k_new.size(2) == d && v_new.sizes() == k_new.sizes() && (d == 128 || d == 256) && h % hk == 0 &&
              h / hk <= 16 && k_pages.size(0) >= 1 && k_pages.size(1) == hk && k_pages.size(2) == 16 && k_pages.size(3) == d && v_pages.sizes() == k_pages.sizes() &&
-             table.size(0) == s && table.size(1) >= 1 && start.size(0) == s + 1 && r <= 65535 && s <= 65535 && h <= 65535 && k_pages.size(0) <= INT32_MAX &&
+             table.size(0) == s && table.size(1) >= 1 && start.size(0) == s + 1 && r <= 65535 && s <= 65535 && h <= 65535 && r * h <= INT32_MAX && k_pages.size(0) <= INT32_MAX &&
              table.size(1) <= INT32_MAX,
          "unsupported attention shape");
     need(plain(q, at::kBFloat16) && plain(k_new, at::kBFloat16) && plain(v_new, at::kBFloat16) && plain(k_pages, at::kBFloat16) && plain(v_pages, at::kBFloat16),

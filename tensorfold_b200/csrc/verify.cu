@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kChoiceThreads, 1) verify_choice_kernel(const 
     pdl_wait();
     const int blocks = cluster.num_blocks(), rank = cluster.block_rank(), seq = blockIdx.x / blocks;
     const int r0 = a.seq_start[seq], n = a.seq_start[seq + 1] - r0;
-    if (n < 1) {                                 // a sequence without rows: the whole cluster leaves
+    if (r0 < 0 || n < 1 || r0 > a.R - n) {       // a sequence without rows, or not among the call's: the whole cluster leaves
         if (rank == 0 && tid == 0) { a.keep[seq] = 0; a.next[seq] = -1; }
         return;
     }

@@ -803,7 +803,8 @@ int run(WindowArgs& a, cudaStream_t st) {
 extern "C" {
 
 int tf_window_slots(int window, int sinks, int max_window, int max_context, int chunk_keys) {
-    if (window < 0 || sinks < 0 || max_window < 1 || max_context < max_window || max_context > (1 << 30) || chunk_keys < tf::kTile || chunk_keys % tf::kTile)
+    if (window < 0 || sinks < 0 || max_window < 1 || max_context < max_window || max_context > (1 << 30) || chunk_keys < tf::kTile || chunk_keys > (1 << 30) ||
+        chunk_keys % tf::kTile)
         return 0;
     const tf::Slots s = tf::slots_for(window, sinks, max_window, max_context, chunk_keys);
     return s.first + s.near;
@@ -831,13 +832,13 @@ int tf_window_attention(const void* q, const void* k_new, const void* v_new, con
     if ((group != 64 && group != 32) || (qg && (qg_stride % 8 || qg_stride < (size_t)heads * 2 * head_dim)) || (out_packed && rows > TF_QMM_MAX_ROWS)) return TF_EINVAL;
     if (rows < 1 || n_seqs < 1 || max_window < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || num_pages < 1 || max_pages < 1) return TF_EINVAL;
     if ((head_dim != 128 && head_dim != 256) || heads / kv_heads > 16 || !(scale > 0.f) || !(scale < INFINITY)) return TF_EINVAL;
+    if (rows > 65535 || kv_heads > 65535 || (long long)rows * heads > 0x7FFFFFFFll || (long long)num_pages * kv_heads * 16 > 0x7FFFFFFFll) return TF_EINVAL;
     const int slots = tf_window_slots(window, sinks, max_window, max_context, chunk_keys);
     if (slots < 1) return TF_EINVAL;
     if (!q || !k_new || !v_new || !k_pages || !v_pages || !page_table || !seq_lens || !seq_start) return TF_EINVAL;
     if (((uintptr_t)q | (uintptr_t)k_new | (uintptr_t)v_new | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)qg | (uintptr_t)out_packed |
          (uintptr_t)out) & 15) return TF_EALIGN;
     if (!scratch || ((uintptr_t)scratch & 15) || scratch_bytes < tf_window_scratch_bytes(rows, heads, head_dim, slots)) return TF_ESCRATCH;
-    if (rows > 65535 || kv_heads > 65535 || (long long)num_pages * kv_heads * 16 > 0x7FFFFFFFll) return TF_EINVAL;
     tf::WindowArgs a{};
     a.q = static_cast<const __nv_bfloat16*>(q);
     a.k_new = static_cast<const __nv_bfloat16*>(k_new); a.v_new = static_cast<const __nv_bfloat16*>(v_new);

@@ -102,7 +102,8 @@ def test_refusals_before_any_launch(lib):
 
     for bad in (dict(rows=0), dict(seqs=0), dict(wide=0), dict(context=1), dict(win=-1), dict(sinks=-1), dict(chunk=32), dict(chunk=100), dict(heads=23), dict(heads=68),
                 dict(d=64), dict(scale=0.0), dict(scale=float("inf")), dict(scale=float("nan")), dict(out=None), dict(q=None), dict(group=16), dict(gate=p, stride=8),
-                dict(pages=0), dict(rows=70000), dict(pages=1 << 30)):
+                dict(pages=0), dict(rows=70000), dict(pages=1 << 30),
+                dict(rows=65000, heads=64000, kv_heads=4000), dict(chunk=(1 << 30) + 64)):
         assert window(**bad) == _lib.TF_EINVAL, bad
     assert window(q=p + 2) == window(out=p + 8) == _lib.TF_EALIGN
     assert window(scratch=None) == window(size=64) == _lib.TF_ESCRATCH

@@ -365,3 +365,81 @@ def test_bounds_are_checked(lib):
     for bad in (dict(window=0), dict(window=5, budget=9), dict(budget=0), dict(budget=10, recent=8, sinks=3), dict(sinks=1), dict(recent=1), dict(window=9, sinks=-1)):
         with pytest.raises(ValueError):
             F.State(w, 1, 64, **bad)
+
+
+def test_offsets_beyond_32_bits(lib):
+    """Pages that lie more than 2^32 values into a cache: the bits of the same pages at its front."""
+
+    from tensorfold_b200 import _lib, lane_evict, lane_window
+
+    h, hk, d, n, w = 4, 1, 256, 90, 3
+    gen = torch.Generator().manual_seed(12)
+    count, used = (1 << 20) + 64, 6                            # 2^32 values of K and as many of V: 8.6 GB each
+    rows, fill = (torch.randn((w, hk, d), generator=gen).to(BF).cuda() for _ in range(2)), torch.randn((2, used, hk, 16, d), generator=gen).to(BF).cuda()
+    rows = list(rows)
+    q = torch.randn((w, h, d), generator=gen).to(BF).cuda()
+    results = []
+    for first, total in ((0, used), (count - used, count)):
+        k, v = torch.empty((1, total, hk, 16, d), dtype=BF, device="cuda"), torch.empty((1, total, hk, 16, d), dtype=BF, device="cuda")
+        k[0, first:], v[0, first:] = fill[0], fill[1]
+        mass, pos = torch.zeros((1, total, hk, 16), device="cuda"), torch.zeros((1, total, hk, 16), dtype=torch.int32, device="cuda")
+        mass[0, first:] = torch.arange(used * 16, device="cuda").reshape(used, 1, 16).flip(0).float()
+        pos[0, first:] = 50
+        table, lens, start = i32([[first + i for i in range(used)]]), i32([n]), i32([0, w])
+        lse = torch.empty((1, w, h), device="cuda")
+        out = lane_window.window_attention(q, *rows, k[0], v[0], table, lens, start, scale=0.1, max_window=w, max_context=n + w, lse=lse[0])
+        lane_evict.attention_mass(q[None], lse, k, table, i32([n - w]), start, i32([w]), i32([7, 8, 9]), mass, pos, scale=0.1, max_window=w, max_context=n)
+        moved = lane_evict.evict(k, v, table, i32([n]), i32([1000]), mass, pos, 40, recent=0, sinks=8, max_context=n)
+        results.append([t.clone() for t in (out, lse, mass[0, first:], pos[0, first:], k[0, first:], v[0, first:], moved)])
+        del k, v
+    for a, b in zip(*results):
+        assert_same_bits(a, b)
+    assert int(results[0][-1]) > 0
+    _lib.status(torch.device("cuda", 0)).raise_if_set()
+    torch.cuda.empty_cache()
+
+
+def test_two_streams_at_once(lib):
+    """Calls of every kind on two streams, with nothing shared: each gives what it gives alone."""
+
+    from tensorfold_b200 import lane_evict, lane_window, speculative
+
+    def rounds(seed, d):
+        gen = torch.Generator().manual_seed(seed)
+        h, hk, s, used = 8, 2, 6, 40
+        k, v = (torch.randn((2, s * used, hk, 16, d), generator=gen).to(BF).cuda() for _ in range(2))
+        mass, pos = torch.rand((2, s * used, hk, 16), generator=gen).cuda(), torch.arange(16).repeat(2, s * used, hk, 1).to(torch.int32).cuda()
+        q, kn, vn = (torch.randn((4 * s, x, d), generator=gen).to(BF).cuda() for x in (h, hk, hk))
+        logits, tokens = torch.randn((4 * s, 5000), generator=gen).to(BF).cuda(), torch.randint(0, 5000, (4 * s,), generator=gen).to(torch.int32).cuda()
+        u = torch.rand((4 * s, 2), generator=gen).cuda()
+        table, lens, start = torch.randperm(s * used, generator=gen).to(torch.int32).reshape(s, used).cuda(), i32([600, 5, 333, 70, 480, 17]), i32(range(0, 4 * s + 1, 4))
+        row_pos = i32([0] * (4 * s))
+        yield
+        for _ in range(6):
+            lse = torch.empty((2, 4 * s, h), device="cuda")
+            outs = [lane_window.window_attention(q, kn, vn, k[i], v[i], table, lens, start, scale=0.08, max_window=4, max_context=640, lse=lse[i]) for i in range(2)]
+            keep, token = speculative.verify_drafts(logits, tokens, start, u, draft_logits=logits.flip(0))
+            lane_evict.attention_mass(torch.stack([q, q]), lse, k, table, lens, start, keep, row_pos, mass, pos, scale=0.08, max_window=4, max_context=640)
+            moved = lane_evict.evict(k, v, table, lens, lens, mass, pos, 300, recent=10, sinks=2, max_context=640)
+            yield
+        yield [*outs, lse, keep, token, mass, pos, k, v, moved]
+
+    def drive(together):
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        runs = [rounds(5, 128), rounds(6, 256)]
+        results = [None, None]
+        for r in runs:
+            next(r)
+        torch.cuda.synchronize()
+        for _ in range(7):
+            for i, (st, r) in enumerate(zip(streams, runs)):
+                with torch.cuda.stream(st):
+                    results[i] = next(r)
+                if not together:
+                    torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return results
+
+    for one, two in zip(drive(False), drive(True)):
+        for a, b in zip(one, two):
+            assert_same_bits(a, b)

@@ -177,6 +177,22 @@ def test_tokens_follow_the_target(lib):
     assert abs(kept / total - rate) <= 5 * math.sqrt(rate * (1 - rate) / total)
 
 
+def test_sequences_that_are_not_among_the_rows(lib):
+    """seq_start lies on the device, where no check of arguments sees it: such a sequence has no rows, the others are as ever."""
+
+    from tensorfold_b200 import speculative
+
+    logits, near, tokens, starts, u = case(9, [4, 2], 3001)
+    dev = [logits.cuda(), tokens.cuda(), None, u.cuda()]
+    right = plain(logits, tokens, starts, u, 1.0, near, 1.0)
+    for bad, which in (([0, 4, 99], 0), ([-3, 4, 6], 1), ([0, 4, 2 ** 31 - 1], 0), ([-2 ** 31, 4, 6], 1)):
+        dev[2] = i32(bad).cuda()
+        keep, nxt = speculative.verify_drafts(*dev, draft_logits=near.cuda())
+        torch.cuda.synchronize()
+        assert keep.tolist()[which] == right[0][which] and nxt.tolist()[which] == right[1][which]
+        assert keep.tolist()[1 - which] == 0 and nxt.tolist()[1 - which] == -1
+
+
 def test_capture_and_refusals(lib):
     from tensorfold_b200 import speculative
 
