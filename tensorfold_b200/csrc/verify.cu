@@ -20,6 +20,8 @@
 
 #include <cooperative_groups.h>
 
+#include <utility>
+
 #include "tc.cuh"
 
 namespace tf {
@@ -367,6 +369,7 @@ __global__ void __launch_bounds__(kChoiceThreads, 1) verify_choice_kernel(const 
         if (total > kZero || mode == kAll) break;
         mode = kAll;                             // at most once: the second pass ends above
     }
+    auto others = cluster.barrier_arrive();      // this block has read what it needs of the others
     // ---- the first token whose cumulative weight is above the goal ----
     if (warp == 0) {
         const double goal = goal_u * total;
@@ -428,7 +431,7 @@ __global__ void __launch_bounds__(kChoiceThreads, 1) verify_choice_kernel(const 
             if (lane == 0) a.next[seq] = token;
         }
     }
-    cluster.sync();                              // nobody leaves while another block may read its sums
+    cluster.barrier_wait(std::move(others));     // nobody leaves while another block may read its sums
 }
 
 // Blocks a sequence: as many as still let all sequences' clusters run at the same time, which the GPU is asked once (of 148 SMs, for
