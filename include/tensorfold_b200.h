@@ -311,7 +311,7 @@ int tf_lane_attention_paged_static(const void* q, const void* k_new, const void*
 /* The same kind of attention with a sliding window and sinks (no counterpart in the reference): row t of sequence s
  * stands at slot p = seq_lens[s] + t and sees key j <= p where p - j < window or j < sinks; window 0: every key up to its own
  * (sinks then change nothing). Keys are cut by absolute position into chunks of chunk_keys (a multiple of 64) that are
- * attended by themselves and joined in order, so a row's bits depend on chunk_keys and on its own keys only. A call's partials
+ * attended by themselves and joined in order (tf_window_chunk_keys: a good size, 0 for bad arguments), so a row's bits depend on chunk_keys and on its own keys only. A call's partials
  * live in `slots` = tf_window_slots(...) chunks of scratch (tf_window_scratch_bytes, 16-byte aligned, no initialisation; calls that overlap
  * on the GPU must not share it). tf_window_launches: how many kernels a call queues: the chunks, before them a plan where blocks take
  * several of them, behind them a join unless there is one slot and the call is plain (neither qg nor out_packed). q, k_new, v_new, pages, out 16-byte aligned. num_pages bounds the page numbers: an entry
@@ -320,6 +320,7 @@ int tf_lane_attention_paged_static(const void* q, const void* k_new, const void*
  * reported). lse, when not NULL, receives ln(sum exp(score)) [rows, heads] fp32. Rows behind seq_start[n_seqs] are left as
  * they were in out and lse. out, qg, out_packed, group: as below for tf_lane_attention_paged_gated. Keys that no row may see (stale
  * rows of a page, later rows) may hold anything; a row that sees a value that is not finite has no specified result. */
+int tf_window_chunk_keys(int n_seqs, int heads, int kv_heads, int max_window, int max_context, int window, int sinks);
 int tf_window_slots(int window, int sinks, int max_window, int max_context, int chunk_keys);
 size_t tf_window_scratch_bytes(int rows, int heads, int head_dim, int slots);
 int tf_window_launches(int rows, int n_seqs, int max_window, int slots, int heads, int kv_heads, int head_dim, int plain);

@@ -83,6 +83,7 @@ SIGNATURES: dict[str, tuple] = {
                                                c_float, c_void_p]),
     "tf_kv_commit": (c_int, [c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_int, c_void_p,
                              c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p]),
+    "tf_window_chunk_keys": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "tf_window_slots": (c_int, [c_int, c_int, c_int, c_int, c_int]),
     "tf_window_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "tf_window_launches": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),

@@ -311,7 +311,7 @@ int32_t checked_int(PyObject* o, const char* text) {
 }
 
 // window_attention(q, k_new, v_new, k_pages, v_pages, page_table, seq_lens, seq_start, scale, max_window, max_context, window (0: none), sinks,
-//                  chunk_keys, scratch, out, lse, gate, packed data, packed group, status) -> out or None
+//                  chunk_keys (0: tf_window_chunk_keys), scratch, out, lse, gate, packed data, packed group, status) -> out or None
 PyObject* window_attention_py(PyObject* const* args, Py_ssize_t n) {
     if (n != 21) fail(PyExc_TypeError, "window_attention takes 21 arguments");
     at::AutoDispatchBelowADInplaceOrView no_grad;
@@ -322,7 +322,7 @@ PyObject* window_attention_py(PyObject* const* args, Py_ssize_t n) {
     const double scale = convert<double>(args[8]);
     const char* sizes = "window >= 1 (or None), sinks >= 0, chunk_keys a positive multiple of 64 and max_context >= max_window >= 1 required";
     const int max_window = checked_int(args[9], sizes), max_context = checked_int(args[10], sizes), window = checked_int(args[11], sizes),
-              sinks = checked_int(args[12], sizes), chunk = checked_int(args[13], sizes), group = convert<int>(args[19]);
+              sinks = checked_int(args[12], sizes), given_chunk = checked_int(args[13], sizes), group = convert<int>(args[19]);
     on_device(q, k_new, v_new, k_pages, v_pages, table, lens, start, lse, gate, packed, out, args[14] == Py_None ? at::Tensor() : tensor(args[14]));
     need(q.dim() == 3 && k_new.dim() == 3 && k_pages.dim() == 4 && table.dim() == 2 && lens.dim() == 1 && start.dim() == 1, "unsupported attention shape");
     const int64_t r = q.size(0), h = q.size(1), d = q.size(2), hk = k_new.size(1), s = lens.size(0);
@@ -335,6 +335,7 @@ PyObject* window_attention_py(PyObject* const* args, Py_ssize_t n) {
          "attention tensors must be contiguous bf16");
     need(plain(table, at::kInt) && plain(lens, at::kInt) && plain(start, at::kInt), "page_table, seq_lens and seq_start must be contiguous int32");
     need(scale > 0 && scale < INFINITY, "scale must be positive and finite");
+    const int chunk = given_chunk != 0 ? given_chunk : tf_window_chunk_keys((int)s, (int)h, (int)hk, max_window, max_context, window, sinks);
     const int slots = tf_window_slots(window, sinks, max_window, max_context, chunk);
     need(slots > 0, sizes);
     need(!lse.defined() || (plain(lse, at::kFloat) && lse.dim() == 2 && lse.size(0) == r && lse.size(1) == h), "lse must be contiguous float32 (R, H)");
@@ -510,7 +511,7 @@ PyMethodDef methods[] = {
     TF_FN(tf_moe_combine_peer, 1), TF_FN(tf_moe_pack, 1), TF_FN(tf_moe_act, 1), TF_FN(tf_moe_combine, 1), TF_FN(tf_peer_slot_bytes, 0),
     TF_FN(tf_peer_exchange, 1), TF_FN(tf_qmm_act, 1), TF_FN(tf_swiglu_tiled, 1), TF_FN(tf_qmm_peer, 1), TF_FN(tf_norm_xs_peer, 1),
     TF_FN(tf_set_poll_limit, 0), TF_FN(tf_topk_scratch_bytes, 0), TF_FN(tf_topk_rows, 2), TF_FN(tf_topk_sample_rows, 2), TF_FN(tf_sample_rows, 1),
-    TF_FN(tf_window_slots, 0), TF_FN(tf_window_scratch_bytes, 0), TF_FN(tf_window_launches, 0),
+    TF_FN(tf_window_chunk_keys, 0), TF_FN(tf_window_slots, 0), TF_FN(tf_window_scratch_bytes, 0), TF_FN(tf_window_launches, 0),
     TF_FN(tf_window_attention, 2), TF_FN(tf_attention_mass, 1),        // (without a plan; window_attention() counts it)
     TF_FN(tf_evict_scratch_bytes, 0), TF_FN(tf_kv_evict, 2), TF_FN(tf_verify_scratch_bytes, 0), TF_FN(tf_verify_rows, 2),
     TF_OWN("bound", bound_py), TF_OWN("scratch", scratch_py), TF_OWN("lane_matmul", lane_matmul_py), TF_OWN("prefill_matmul", prefill_matmul_py),

@@ -802,6 +802,37 @@ int run(WindowArgs& a, cudaStream_t st) {
 
 extern "C" {
 
+// Few columns (sequence, KV head, group of up to 128 query rows): as many chunks as leave the SMs one each, but not below the size at
+// which a chunk's tiles (0.95 us for 64 keys) and the join (0.36 us a chunk) cost the same, and one chunk where that saves the join for few
+// tiles more (300 rows of up to 400 keys: 15.2 us in one, 19.7 in two). More columns: a quarter of what a group sees, so that the chunks
+// can be dealt out evenly (16 x 4 columns of 4100 keys: 59.1 us in chunks of 1024, 59.6 of 2048, 64.8 of 512, 77 of 4096; with heads of
+// 128 38.7, 48.7, 43.3 and 71.6). Very many, as for a prompt's rows: one chunk, without partials and join, where a group sees few
+// keys (362 columns of 1040 keys: 45.5 us, 57 in chunks of 2048; 576 of 4000: 222 and 284), else 2048 (376 columns of 17500 keys:
+// 511 us, 643 in one chunk, whose columns do not divide evenly).
+int tf_window_chunk_keys(int n_seqs, int heads, int kv_heads, int max_window, int max_context, int window, int sinks) {
+    if (n_seqs < 1 || kv_heads < 1 || heads < kv_heads || heads / kv_heads > tf::kRows || max_window < 1 || max_context < max_window ||
+        max_context > (1 << 30) || window < 0 || sinks < 0) return 0;
+    const auto over = [](long long x, long long y) { return (x + y - 1) / y; };
+    const auto tiles_of = [&](long long keys) { return over(keys, tf::kTile) * tf::kTile; };
+    const int most = tf::kRows / (heads / kv_heads), rows = max_window < most ? max_window : most;
+    const long long columns = (long long)n_seqs * kv_heads * over(max_window, rows);
+    const long long seen = (long long)window + rows - 1, keys = window == 0 || seen > max_context ? max_context : seen;
+    const long long whole = tiles_of(max_context < 128 ? 128 : max_context);
+    const long long spare = tf::kSms / columns - (window == 0 ? 0 : sinks > 0 ? 2 : 1);     // a window lies across one chunk more, sinks have their own
+    long long chunk = 128;
+    if (spare >= 1) {
+        const long long even = (long long)sqrt(24.0 * keys), share = over(keys, spare);
+        chunk = tiles_of(even > share ? even > 128 ? even : 128 : share > 128 ? share : 128);
+        if (whole - chunk <= 256) chunk = whole;
+    } else if (columns < 222) {
+        chunk = tiles_of(over(keys, 4));
+        chunk = chunk < 512 ? 512 : chunk > 2048 ? 2048 : chunk;
+    } else {
+        chunk = keys <= 4096 ? whole : 2048;
+    }
+    return (int)(chunk > 1 << 30 ? 1 << 30 : chunk);
+}
+
 int tf_window_slots(int window, int sinks, int max_window, int max_context, int chunk_keys) {
     if (window < 0 || sinks < 0 || max_window < 1 || max_context < max_window || max_context > (1 << 30) || chunk_keys < tf::kTile || chunk_keys > (1 << 30) ||
         chunk_keys % tf::kTile)
