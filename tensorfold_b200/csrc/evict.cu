@@ -95,11 +95,12 @@ __global__ void __launch_bounds__(kMassThreads, 1) mass_kernel(const __grid_cons
     if (warp == kMassLoad) {
         const int* pt = a.page_table + (size_t)seq * a.max_pages;
         Ring ring(KS, 1);
-        // a tile's eight pages, a lane each, looked up a tile ahead; one behind the last key or that is none (reported) is copied from
-        // page 0 and not used
+        // a lane copies 64 values of a page's 16 rows, the lanes of a page beside one another; page numbers are looked up a tile ahead; one
+        // behind the last key or that is none (reported) is copied from page 0 and not used
+        const int slab = lane % C::SLABS, at = lane / C::SLABS;
         auto number = [&](int t) -> int {
-            const int j = t * kMassKeys + lane * kPage;
-            if (lane >= 8 || t >= last || j >= keys) return 0;
+            const int j = t * kMassKeys + at * kPage;
+            if (at >= 8 || t >= last || j >= keys) return 0;
             const int page = pt[j / kPage];
             if (page >= 0 && page < a.num_pages) return page;
             report(a.status, TF_EINVAL);
@@ -112,11 +113,9 @@ __global__ void __launch_bounds__(kMassThreads, 1) mass_kernel(const __grid_cons
             wait(k_empty(ring.i), ring.phase);
             if (lane == 0) mbar_arrive_expect_tx(k_full(ring.i), C::TILE_BYTES);
             __syncwarp();
-            if (lane < 8) {
+            if (at < 8) {
                 const int y = ((layer * a.num_pages + page) * a.HK + kvh) * kPage;
-                const uint32_t to = smem_u32(k_s) + ring.i * C::TILE_BYTES + lane * (kPage * 128);
-#pragma unroll
-                for (int c = 0; c < C::SLABS; ++c) tma_4d(to + c * C::K_SLAB, &k_map, 0, y, c, 0, k_full(ring.i));
+                tma_4d(smem_u32(k_s) + ring.i * C::TILE_BYTES + slab * C::K_SLAB + at * (kPage * 128), &k_map, 0, y, slab, 0, k_full(ring.i));
             }
             __syncwarp();
             ring.next();
