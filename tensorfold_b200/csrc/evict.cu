@@ -253,27 +253,28 @@ struct EvictArgs {
     int num_pages, max_pages, HK, S, budget, recent, sinks, max_context, most;
 };
 
-// Exclusive prefix sum over the block (kSelThreads threads) of two counts below 2^32 packed in one word; `total`: the sum.
-__device__ __forceinline__ unsigned long long block_scan(unsigned long long v, unsigned long long* warp_s, unsigned long long& total) {
+// Exclusive prefix sum over the block (kSelThreads threads) of counts (two below 2^32 in a 64-bit word); `total`: the sum. The warps' sums are scanned by
+// every warp for itself.
+template <class T>
+__device__ __forceinline__ T block_scan(T v, unsigned long long* warp_s, T& total) {
+    static_assert(kSelThreads == 32 * 32, "a lane a warp");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    unsigned long long x = v;
+    auto inclusive = [&](T x) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-    }
+        for (int o = 1; o < 32; o <<= 1) {
+            const T y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        return x;
+    };
+    const T x = inclusive(v);
     __syncthreads();                  // an earlier scan's sums have been read
     if (lane == 31) warp_s[warp] = x;
     __syncthreads();
-    unsigned long long before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kSelThreads / 32; ++w) {
-        const unsigned long long s = warp_s[w];
-        before += w < warp ? s : 0;
-        total += s;
-    }
-    return before + x - v;
+    const T sums = inclusive((T)warp_s[lane]);
+    total = __shfl_sync(0xffffffffu, sums, 31);
+    const T before = __shfl_sync(0xffffffffu, sums, (warp + 31) & 31);
+    return (warp > 0 ? before : 0) + x - v;
 }
 
 // Bound by its chain of dependent steps (4224 slots: 12.9 us with 64 of them on the GPU): the page numbers, then weights and positions, a
@@ -377,8 +378,8 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
             }
             // thread i holds bins 2047 - 2i and 2046 - 2i: prefix sums from the largest digit down
             const unsigned c0 = hist[kBins - 1 - 2 * tid], c1 = hist[kBins - 2 - 2 * tid];
-            unsigned long long total;
-            const unsigned before = (unsigned)block_scan(c0 + c1, warp_s, total);
+            unsigned all;
+            const unsigned before = block_scan(c0 + c1, warp_s, all);
             if (before < need && before + c0 >= need) { digit_s = kBins - 1 - 2 * tid; above_s = before; }
             else if (before + c0 < need && before + c0 + c1 >= need) { digit_s = kBins - 2 - 2 * tid; above_s = before + c0; }
             __syncthreads();
@@ -389,11 +390,11 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
     // kept: every key above `prefix` and the first `need` slots of that key. Each thread takes a run of slots (an odd number of
     // words: no bank conflicts)
     const int per = ((n + kSelThreads - 1) / kSelThreads) | 1, lo = min(n, tid * per), hi = min(n, lo + per);
-    unsigned long long counts = 0, total;
-    for (int j = lo; j < hi; ++j) counts += key(j) == prefix;
-    const unsigned eq0 = (unsigned)block_scan(counts, warp_s, total);
+    unsigned equal = 0, all_equal;
+    for (int j = lo; j < hi; ++j) equal += key(j) == prefix;
+    const unsigned eq0 = block_scan(equal, warp_s, all_equal);
     unsigned eq = eq0;
-    counts = 0;                                  // holes below the budget | kept slots above it
+    unsigned long long counts = 0, total;        // holes below the budget | kept slots above it
     for (int j = lo; j < hi; ++j) {
         const uint32_t k = key(j);
         const bool kept = k > prefix || (k == prefix && eq++ < need);

@@ -208,7 +208,7 @@ enum Weights { kAll, kWithout, kResidual };     // p; p without the draft; max(p
 
 __global__ void __launch_bounds__(kChoiceThreads, 1) verify_choice_kernel(const VerifyArgs a) {
     // sums of the block's spans: [0] p, [1] q, then the weights of the first and the second attempt; of its segments; of every block's spans
-    __shared__ double table[kTable], table_p[kTable], table_q[kTable], span_s[4][kMost], seg[2 * kMost * kSpan], all_s[kMaxSpans];
+    __shared__ double table[kTable], table_p[kTable], table_q[kTable], span_s[4][kMost], seg[2 * kMost * kSpan], all_s[2][kMaxSpans];
     __shared__ float offset_s[2][kKept];         // target's and drafter's, of the window's first rows
     __shared__ int first_out;
     cg::cluster_group cluster = cg::this_cluster();
@@ -273,17 +273,29 @@ __global__ void __launch_bounds__(kChoiceThreads, 1) verify_choice_kernel(const 
     const int held_at = tid - holder * least - min(holder, more);
     const Weight target(a.c64, op, a.most, table_p), drafted(a.draft_c64, oq, a.draft_most, table_q);
     auto load_q = [&](int c, float (&v)[8]) { unpack8(abreast ? q.raw(c) : q.edge(p.first(c)), v); };
-    // the sum over all spans of the cluster, `which` of the span sums, in order; all_s keeps them. The whole block; the clusters' span sums are
-    // complete (a cluster barrier lies before).
-    auto gather = [&](int which) -> double {
+    // the sums over all spans of the cluster, in order, of `which` of the span sums and (two) of the next; all_s keeps them. The whole
+    // block; the clusters' span sums are complete (a cluster barrier lies before).
+    auto gather = [&](int which, bool two, double& second) -> double {
         static_assert(kMaxSpans <= kChoiceThreads, "a thread a span");
         __syncthreads();                         // all_s is no longer read
-        if (tid < spans) all_s[tid] = cluster.map_shared_rank(&span_s[which][0], holder)[held_at];
+        if (tid < spans) {
+            const double* from = cluster.map_shared_rank(&span_s[which][held_at], holder);
+            const double x = from[0], y = two ? from[kMost] : 0.0;
+            all_s[0][tid] = x;
+            if (two) all_s[1][tid] = y;
+        }
         __syncthreads();
         double sum = 0.0;
-        for (int i = lane; i < spans; i += 32) sum += all_s[i];
+        second = 0.0;
+        for (int i = lane; i < spans; i += 32) {
+            sum += all_s[0][i];
+            if (two) second += all_s[1][i];
+        }
 #pragma unroll
-        for (int k = 16; k; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+        for (int k = 16; k; k >>= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, k);
+            if (two) second += __shfl_xor_sync(0xffffffffu, second, k);
+        }
         return sum;
     };
     if (mode == kResidual) {
@@ -311,7 +323,8 @@ __global__ void __launch_bounds__(kChoiceThreads, 1) verify_choice_kernel(const 
             span_s[i < mine ? 0 : 1][i < mine ? i : i - mine] = sum;
         }
         cluster.sync();
-        const double zp = gather(0), zq = gather(1);
+        double zq;
+        const double zp = gather(0, true, zq);
         // the normalisers go into the tables; a drafter without any probability takes nothing off (2^-900 a token)
         if (tid < kTable) {
             const double whole = exp2(tid / (double)kTable);
@@ -341,7 +354,7 @@ __global__ void __launch_bounds__(kChoiceThreads, 1) verify_choice_kernel(const 
                 if (i + e == x) w[e] = 0.0;
         }
     };
-    double total;
+    double total, unused;
     for (int attempt = 0;; ++attempt) {
         for (int s = warp; s < segs; s += kChoiceWarps) {
             double sum = 0.0;
@@ -364,7 +377,7 @@ __global__ void __launch_bounds__(kChoiceThreads, 1) verify_choice_kernel(const 
             span_s[2 + attempt][i] = sum;
         }
         cluster.sync();
-        total = gather(2 + attempt);
+        total = gather(2 + attempt, false, unused);
         // nothing is left where p is nowhere above q but for rounding, or all of it is on the refused draft: p itself
         if (total > kZero || mode == kAll) break;
         mode = kAll;                             // at most once: the second pass ends above
@@ -400,7 +413,7 @@ __global__ void __launch_bounds__(kChoiceThreads, 1) verify_choice_kernel(const 
             return last_with;
         };
         double at = goal;
-        const int span = search(all_s, spans, at);
+        const int span = search(all_s[0], spans, at);
         if (span < 0) {
             if (rank == 0 && lane == 0) a.next[seq] = -1;        // a row without any probability
         } else if (span >= first && span < first + mine) {
