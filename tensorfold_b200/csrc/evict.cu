@@ -239,8 +239,9 @@ __global__ void __launch_bounds__(kMassThreads, 1) mass_kernel(const __grid_cons
 
 // ---- eviction ------------------------------------------------------------------------------------------
 constexpr int kSelThreads = 1024;
-constexpr int kBins = 2048;
-constexpr int kSelKeys = 49152;      // slots whose keys fit the block's shared memory; longer sequences are ranked from global memory
+constexpr int kBins = 8192;          // of the first histogram: 13 bits of a key; then 10 and 9 bits where many share those
+constexpr int kRanked = kSelThreads / 4;
+constexpr int kSelKeys = 45056;      // slots whose keys fit the block's shared memory; longer sequences are ranked from global memory
 
 struct EvictArgs {
     __nv_bfloat16 *k_pages, *v_pages;   // [layers, pages, HK, 16, D]
@@ -283,14 +284,15 @@ __device__ __forceinline__ T block_scan(T v, unsigned long long* warp_s, T& tota
 template <bool STAGED>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictArgs a) {
     extern __shared__ uint32_t keys_s[];
-    __shared__ unsigned hist[kBins];
+    __shared__ __align__(16) unsigned hist[kBins];
+    __shared__ unsigned long long ranked_s[kRanked];
     __shared__ unsigned long long warp_s[kSelThreads / 32];
-    __shared__ unsigned digit_s, above_s, safe_s;
+    __shared__ unsigned digit_s, above_s, safe_s, count_s;
     pdl_launch_dependents();
     const int kvh = blockIdx.x, seq = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x;
     const size_t item = ((size_t)layer * a.S + seq) * a.HK + kvh;
     for (int b = tid; b < kBins; b += kSelThreads) hist[b] = 0;
-    if (tid == 0) safe_s = 0;
+    if (tid == 0) safe_s = count_s = 0;
     pdl_wait();
     const int L = a.seq_lens[seq], n = min(L, min(a.max_context, a.max_pages * kPage)), safe_from = a.next_pos[seq] - a.recent;
     if (L > n && tid == 0) report(a.status, TF_EINVAL);
@@ -345,7 +347,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
                     const uint32_t r = page[k] < 0 ? 0u : rank_of(mk[e], pk[e]);
                     keys_s[j + e] = r;
                     if (r == kSafe) ++safe;
-                    else atomicAdd(&hist[r >> 21], 1u);
+                    else atomicAdd(&hist[r >> 19], 1u);
                 }
             }
         }
@@ -353,46 +355,80 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
         for (int j = tid; j < n; j += kSelThreads) {
             const uint32_t r = key(j);
             if (r == kSafe) ++safe;
-            else atomicAdd(&hist[r >> 21], 1u);
+            else atomicAdd(&hist[r >> 19], 1u);
         }
     }
     safe = __reduce_add_sync(0xffffffffu, safe);
     if ((tid & 31) == 0 && safe) atomicAdd(&safe_s, safe);
     __syncthreads();
-    // the smallest key that stays, 11 + 11 + 10 bits at a time: the need-th largest of those that are not protected. More protected slots than
-    // the budget holds (positions that are none): the first of them stay
+    // the smallest key that stays: the need-th largest of those that are not protected. More protected slots than the budget holds (positions that
+    // are none): the first of them stay
     uint32_t prefix = kSafe, need = a.budget;
+    bool ties = true;
     if (safe_s < need) {
         need -= safe_s;
-        prefix = 0;
-        for (int pass = 0; pass < 3; ++pass) {
-            const int bits = pass == 2 ? 10 : 11, shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-            if (pass > 0) {
-                for (int b = tid; b < kBins; b += kSelThreads) hist[b] = 0;
+        // thread i holds bins 8191 - 8 i .. 8184 - 8 i: prefix sums from the largest digit down
+        const uint4 *eight = reinterpret_cast<const uint4*>(hist + kBins - 8 - 8 * tid), hi4 = eight[1], lo4 = eight[0];
+        const unsigned bins[8] = {hi4.w, hi4.z, hi4.y, hi4.x, lo4.w, lo4.z, lo4.y, lo4.x};
+        unsigned mine = 0, all;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) mine += bins[x];
+        unsigned before = block_scan(mine, warp_s, all);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            if (before < need && before + bins[x] >= need) { digit_s = kBins - 1 - 8 * tid - x; above_s = before; }
+            before += bins[x];
+        }
+        __syncthreads();
+        prefix = digit_s;
+        need -= above_s;
+        const unsigned many = hist[prefix];
+        if (STAGED && many <= kRanked) {
+            // few enough to be ranked by comparing all with all, four threads a slot; the key becomes the decision
+            for (int j = tid; j < n; j += kSelThreads) {
+                const uint32_t k = keys_s[j];
+                if (k >> 19 == prefix && k != kSafe) ranked_s[atomicAdd(&count_s, 1u)] = (unsigned long long)k << 32 | ~(uint32_t)j;
+            }
+            __syncthreads();
+            const unsigned long long own = (tid >> 2) < many ? ranked_s[tid >> 2] : 0;
+            unsigned above = 0;
+            for (unsigned i = tid & 3; i < many; i += 4) above += ranked_s[i] > own;
+            above += __shfl_xor_sync(0xffffffffu, above, 1);
+            above += __shfl_xor_sync(0xffffffffu, above, 2);
+            if ((tid >> 2) < many && (tid & 3) == 0) keys_s[~(uint32_t)own] = above < need ? kSafe : 0u;
+            __syncthreads();
+            prefix = prefix << 19 | 0x7FFFFu;
+            need = 0;
+            ties = false;
+        } else {
+            for (int pass = 0; pass < 2; ++pass) {
+                const int bits = pass == 0 ? 10 : 9, shift = pass == 0 ? 9 : 0;
+                __syncthreads();                 // the bins have been read
+                hist[tid] = 0;
                 __syncthreads();
                 for (int j = tid; j < n; j += kSelThreads) {
                     const uint32_t k = key(j);
                     if ((k >> (shift + bits)) == prefix && k != kSafe) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
                 }
                 __syncthreads();
+                const unsigned c = hist[kSelThreads - 1 - tid];
+                const unsigned higher = block_scan(c, warp_s, all);
+                if (higher < need && higher + c >= need) { digit_s = kSelThreads - 1 - tid; above_s = higher; }
+                __syncthreads();
+                prefix = prefix << bits | digit_s;
+                need -= above_s;
             }
-            // thread i holds bins 2047 - 2i and 2046 - 2i: prefix sums from the largest digit down
-            const unsigned c0 = hist[kBins - 1 - 2 * tid], c1 = hist[kBins - 2 - 2 * tid];
-            unsigned all;
-            const unsigned before = block_scan(c0 + c1, warp_s, all);
-            if (before < need && before + c0 >= need) { digit_s = kBins - 1 - 2 * tid; above_s = before; }
-            else if (before + c0 < need && before + c0 + c1 >= need) { digit_s = kBins - 2 - 2 * tid; above_s = before + c0; }
-            __syncthreads();
-            prefix = prefix << bits | digit_s;
-            need -= above_s;
         }
     }
     // kept: every key above `prefix` and the first `need` slots of that key. Each thread takes a run of slots (an odd number of
     // words: no bank conflicts)
     const int per = ((n + kSelThreads - 1) / kSelThreads) | 1, lo = min(n, tid * per), hi = min(n, lo + per);
-    unsigned equal = 0, all_equal;
-    for (int j = lo; j < hi; ++j) equal += key(j) == prefix;
-    const unsigned eq0 = block_scan(equal, warp_s, all_equal);
+    unsigned eq0 = 0;
+    if (ties) {
+        unsigned all;
+        for (int j = lo; j < hi; ++j) eq0 += key(j) == prefix;
+        eq0 = block_scan(eq0, warp_s, all);
+    }
     unsigned eq = eq0;
     unsigned long long counts = 0, total;        // holes below the budget | kept slots above it
     for (int j = lo; j < hi; ++j) {
