@@ -278,9 +278,9 @@ __device__ __forceinline__ T block_scan(T v, unsigned long long* warp_s, T& tota
     return (warp > 0 ? before : 0) + x - v;
 }
 
-// Bound by its chain of dependent steps (4224 slots: 12.9 us with 64 of them on the GPU): the page numbers, then weights and positions, a
-// quarter page a thread; three histogram passes over the keys in shared memory, in which the slots that stay anyway take no part; one
-// pass that counts, one that writes.
+// Bound by its chain of dependent steps (64 blocks of 4224 slots: 8.2 us): the page numbers, then weights and positions, a quarter page a
+// thread; a histogram of the keys' first 13 bits, in which the slots that stay anyway take no part; the slots that share those bits with the
+// threshold, few as a rule, ranked by comparison (two more histograms in their place: 10 us); a pass that counts, one that writes.
 template <bool STAGED>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictArgs a) {
     extern __shared__ uint32_t keys_s[];
