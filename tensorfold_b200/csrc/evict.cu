@@ -25,7 +25,7 @@ struct MassArgs {
     float* mass;                   // [layers, pages, HK, 16]
     int* pos;
     int* status;
-    int num_pages, max_pages, H, HK, R, S, max_context;
+    int num_pages, max_pages, H, HK, R, S, layers, max_context;
     float scale_log2;
 };
 
@@ -33,9 +33,11 @@ struct MassArgs {
 // time, the B operand, so that a key's scores lie in one thread's lane and its sum needs no shuffle and no atomic: thread = key, columns
 // in row order, fp32. K arrives a page at a time by tiled copies; slots behind the last key are never added.
 //
-// A block walks the tiles of one (layer, sequence, KV head) that are its share, the row chunks inner: with up to 128 rows (the usual
-// case) Q is staged once. What bounds it: the bytes of K, and 2^x on the special-function units (16 a cycle and SM): a tile's 128 x 48 weights
-// take 400 cycles, its 64 KB 1.5 us at the SM's share of the memory's rate.
+// The tiles of all (layer, KV head, sequence) columns form one sequence that is cut into equal runs, one a block: a block starts in the middle of a
+// column and goes on into the next ones, its copies running ahead over the border. With up to 128 rows (the usual case) Q is staged once a
+// column. What bounds it: the bytes of K (4 layers x 4 heads x 16 users of 2048 to 8192 keys: 767 MB in 135 us, 5.7 TB/s; with blocks that each took
+// a share of one column, three rounds of them, 151 us); 2^x on the special-function units takes a quarter of a tile's 1.5 us. One user of 4096
+// keys in 16 layers: 134 MB in 28 us, of which a block's start is 4.
 constexpr int kMassKeys = 128, kMassRows = 128, kMassSum = 4, kMassMma = 4, kMassLoad = 5, kMassThreads = 6 * 32;
 
 template <int D>
@@ -63,20 +65,6 @@ __global__ void __launch_bounds__(kMassThreads, 1) mass_kernel(const __grid_cons
     auto s_full = [&](int s) { return bars + 8u * (2 * KS + s); };
     auto s_empty = [&](int s) { return bars + 8u * (2 * KS + 2 + s); };
     const uint32_t q_full = bars + 8u * (2 * KS + 4), q_empty = q_full + 8;
-    pdl_wait();
-    // ---- the block's share of the tiles of (layer, sequence, KV head) ----
-    const int kvh = blockIdx.y, layer = blockIdx.z / a.S, seq = blockIdx.z - layer * a.S, G = a.H / a.HK;
-    const int r0 = a.seq_start[seq], n = a.seq_start[seq + 1] - r0, L = a.seq_lens[seq];
-    int kept = min(max(a.keep[seq], 0), n);
-    if (kept < 1) return;
-    if (r0 < 0 || r0 + n > a.R || L < 0 || L > a.max_context - kept || L > a.max_pages * kPage - kept) {      // not what the call was made for
-        if (tid == 0) report(a.status, TF_EINVAL);
-        return;
-    }
-    const int keys = L + kept, tiles = (keys + kMassKeys - 1) / kMassKeys;
-    const int per = (tiles + gridDim.x - 1) / gridDim.x, first = blockIdx.x * per, last = min(tiles, first + per);
-    if (first >= last) return;
-    const int rows = kept * G, chunks = (rows + kMassRows - 1) / kMassRows;
     if (tid == 0) {
         for (int s = 0; s < KS; ++s) { mbar_init(k_full(s), 1); mbar_init(k_empty(s), 1); }
         for (int s = 0; s < 2; ++s) { mbar_init(s_full(s), 1); mbar_init(s_empty(s), kMassSum); }
@@ -91,141 +79,203 @@ __global__ void __launch_bounds__(kMassThreads, 1) mass_kernel(const __grid_cons
     tc_fence_after();
     const uint32_t tmem = tmem_s;
     Waits wait(a.status);
+    pdl_wait();
+    // ---- the block's share of the tiles (it may have none) ----
+    const int G = a.H / a.HK;
+    // sequence s: first row, rows kept, length before the commit, tiles (0: not what the call was made for, reported, or nothing kept)
+    auto column = [&](int s) -> int4 {
+        if (s >= a.S) return make_int4(0, 0, 0, 0);
+        const int r0 = a.seq_start[s], n = a.seq_start[s + 1] - r0, L = a.seq_lens[s], kept = min(max(a.keep[s], 0), n);
+        if (kept < 1) return make_int4(0, 0, 0, 0);
+        if (r0 < 0 || r0 > a.R - n || L < 0 || L > a.max_context - kept || L > a.max_pages * kPage - kept) {
+            report(a.status, TF_EINVAL);
+            return make_int4(0, 0, 0, 0);
+        }
+        return make_int4(r0, kept, L, (L + kept + kMassKeys - 1) / kMassKeys);
+    };
+    long long a_head = 0;                        // tiles of one (layer, KV head)
+    for (int s0 = 0; s0 < a.S; s0 += 32) a_head += __reduce_add_sync(0xffffffffu, (unsigned)column(s0 + lane).w);
+    const long long all = a_head * a.HK * a.layers;
+    const long long begin = all * blockIdx.x / gridDim.x, end = all * (blockIdx.x + 1) / gridDim.x;
+    struct Run {                                 // tiles first .. last - 1 of a column
+        int layer, kvh, seq, r0, kept, L, keys, first, last;
+    };
+    // the block's run that starts at tile `x` of all. Whole warps; the columns are read again, from the cache
+    auto run_at = [&](long long x) -> Run {
+        const int head = (int)(x / a_head);
+        long long left = x - head * a_head;
+        Run r{head / a.HK, head % a.HK, 0, 0, 0, 0, 0, 0, 0};
+        for (int s0 = 0; s0 < a.S; s0 += 32) {
+            const int4 c = column(s0 + lane);
+            int upto = c.w;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += y;
+            }
+            const unsigned m = __ballot_sync(0xffffffffu, upto > left);
+            if (m == 0) {
+                left -= __shfl_sync(0xffffffffu, upto, 31);
+                continue;
+            }
+            const int who = __ffs(m) - 1, tiles = __shfl_sync(0xffffffffu, c.w, who);
+            r.seq = s0 + who;
+            r.r0 = __shfl_sync(0xffffffffu, c.x, who);
+            r.kept = __shfl_sync(0xffffffffu, c.y, who);
+            r.L = __shfl_sync(0xffffffffu, c.z, who);
+            r.keys = r.L + r.kept;
+            r.first = (int)(left - (__shfl_sync(0xffffffffu, upto, who) - tiles));
+            r.last = end - x < tiles - r.first ? r.first + (int)(end - x) : tiles;
+            break;
+        }
+        return r;
+    };
 
     if (warp == kMassLoad) {
-        const int* pt = a.page_table + (size_t)seq * a.max_pages;
         Ring ring(KS, 1);
         // a lane copies 64 values of a page's 16 rows, the lanes of a page beside one another; page numbers are looked up a tile ahead; one
         // behind the last key or that is none (reported) is copied from page 0 and not used
         const int slab = lane % C::SLABS, at = lane / C::SLABS;
-        auto number = [&](int t) -> int {
-            const int j = t * kMassKeys + at * kPage;
-            if (at >= 8 || t >= last || j >= keys) return 0;
-            const int page = pt[j / kPage];
-            if (page >= 0 && page < a.num_pages) return page;
-            report(a.status, TF_EINVAL);
-            return 0;
-        };
-        int next = number(first);
-        for (int t = first; t < last; ++t) {
-            const int page = next;
-            next = number(t + 1);
-            wait(k_empty(ring.i), ring.phase);
-            if (lane == 0) mbar_arrive_expect_tx(k_full(ring.i), C::TILE_BYTES);
-            __syncwarp();
-            if (at < 8) {
-                const int y = ((layer * a.num_pages + page) * a.HK + kvh) * kPage;
-                tma_4d(smem_u32(k_s) + ring.i * C::TILE_BYTES + slab * C::K_SLAB + at * (kPage * 128), &k_map, 0, y, slab, 0, k_full(ring.i));
+        for (long long x = begin; x < end;) {
+            const Run w = run_at(x);
+            x += w.last - w.first;
+            const int* pt = a.page_table + (size_t)w.seq * a.max_pages;
+            auto number = [&](int t) -> int {
+                const int j = t * kMassKeys + at * kPage;
+                if (at >= 8 || t >= w.last || j >= w.keys) return 0;
+                const int page = pt[j / kPage];
+                if (page >= 0 && page < a.num_pages) return page;
+                report(a.status, TF_EINVAL);
+                return 0;
+            };
+            int next = number(w.first);
+            for (int t = w.first; t < w.last; ++t) {
+                const int page = next;
+                next = number(t + 1);
+                wait(k_empty(ring.i), ring.phase);
+                if (lane == 0) mbar_arrive_expect_tx(k_full(ring.i), C::TILE_BYTES);
+                __syncwarp();
+                if (at < 8) {
+                    const int y = ((w.layer * a.num_pages + page) * a.HK + w.kvh) * kPage;
+                    tma_4d(smem_u32(k_s) + ring.i * C::TILE_BYTES + slab * C::K_SLAB + at * (kPage * 128), &k_map, 0, y, slab, 0, k_full(ring.i));
+                }
+                __syncwarp();
+                ring.next();
             }
-            __syncwarp();
-            ring.next();
         }
     } else if (warp == kMassMma) {
         const bool leader = elect_one();
         const uint32_t q_lo = desc_lo(smem_u32(q_s), 1);
         Ring kr(KS, 0), qr(1, 0), sr(2, 1);
-        const int mine = __reduce_max_sync(0xffffffffu, last - first), parts = __reduce_max_sync(0xffffffffu, chunks);
-        const int least = __reduce_max_sync(0xffffffffu, rows);
-        for (int t = 0; t < mine; ++t) {
-            wait(k_full(kr.i), kr.phase);
-            const uint32_t k_lo = desc_lo(smem_u32(k_s) + kr.i * C::TILE_BYTES, 1);
-            for (int c = 0; c < parts; ++c) {
-                if (parts > 1 || t == 0) {
-                    wait(q_full, qr.phase);
-                    qr.next();
-                }
-                wait(s_empty(sr.i), sr.phase);
-                tc_fence_after();
-                // columns in sixteens (N of the tensor core with M = 128)
-                const uint32_t idesc = tc_idesc((min(kMassRows, least - c * kMassRows) + 15) & ~15, false);
+        for (long long x = begin; x < end;) {
+            const Run w = run_at(x);
+            x += w.last - w.first;
+            const int mine = __reduce_max_sync(0xffffffffu, w.last - w.first), least = __reduce_max_sync(0xffffffffu, w.kept * G);
+            const int parts = (least + kMassRows - 1) / kMassRows;
+            for (int t = 0; t < mine; ++t) {
+                wait(k_full(kr.i), kr.phase);
+                const uint32_t k_lo = desc_lo(smem_u32(k_s) + kr.i * C::TILE_BYTES, 1);
+                for (int c = 0; c < parts; ++c) {
+                    if (parts > 1 || t == 0) {
+                        wait(q_full, qr.phase);
+                        qr.next();
+                    }
+                    wait(s_empty(sr.i), sr.phase);
+                    tc_fence_after();
+                    // columns in sixteens (N of the tensor core with M = 128)
+                    const uint32_t idesc = tc_idesc((min(kMassRows, least - c * kMassRows) + 15) & ~15, false);
 #pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks)
-                    tc_mma_ss(leader, tmem + sr.i * kMassRows, k_lo + (((ks >> 2) * C::K_SLAB + (ks & 3) * 32) >> 4), q_lo + (((ks >> 2) * C::Q_SLAB + (ks & 3) * 32) >> 4), idesc,
-                              ks > 0);
-                if (leader) {
-                    tc_commit(s_full(sr.i));
-                    if (parts > 1) tc_commit(q_empty);
-                    if (c + 1 == parts) tc_commit(k_empty(kr.i));
+                    for (int ks = 0; ks < D / 16; ++ks)
+                        tc_mma_ss(leader, tmem + sr.i * kMassRows, k_lo + (((ks >> 2) * C::K_SLAB + (ks & 3) * 32) >> 4), q_lo + (((ks >> 2) * C::Q_SLAB + (ks & 3) * 32) >> 4),
+                                  idesc, ks > 0);
+                    if (leader) {
+                        tc_commit(s_full(sr.i));
+                        if (parts > 1 || t + 1 == mine) tc_commit(q_empty);
+                        if (c + 1 == parts) tc_commit(k_empty(kr.i));
+                    }
+                    __syncwarp();
+                    sr.next();
                 }
-                __syncwarp();
-                sr.next();
+                kr.next();
             }
-            kr.next();
         }
     } else {
         const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-        const size_t plane = (size_t)layer * a.num_pages * a.HK * kPage;
-        const int* pt = a.page_table + (size_t)seq * a.max_pages;
         Ring sr(2, 0), qr(1, 1);
-        auto stage = [&](int c) {            // rows c * 128 ..: into shared memory, with their log-sum-exps
-            const int q0 = c * kMassRows, count = min(kMassRows, rows - q0);
-            const size_t row0 = (size_t)layer * a.R + r0;
-            constexpr int B = 8, STEP = kMassSum * 32;       // loads in flight a thread
-            for (int e0 = tid; e0 < count * CPR; e0 += B * STEP) {
-                uint4 v[B];
-#pragma unroll
-                for (int k = 0; k < B; ++k) {
-                    const int e = min(e0 + k * STEP, count * CPR - 1), r = e / CPR, x = e % CPR, t = (q0 + r) / G;
-                    v[k] = *reinterpret_cast<const uint4*>(a.q + ((row0 + t) * a.H + kvh * G + q0 + r - t * G) * D + x * 8);
-                }
-#pragma unroll
-                for (int k = 0; k < B; ++k) {
-                    const int e = e0 + k * STEP, r = e / CPR, x = e % CPR;
-                    if (e < count * CPR) *reinterpret_cast<uint4*>(q_s + (x >> 3) * C::Q_SLAB + r * 128 + (((x ^ r) & 7) << 4)) = v[k];
-                }
-            }
-            if (tid < count) {
-                const int t = (q0 + tid) / G;
-                lse_s[tid] = a.lse[(row0 + t) * a.H + kvh * G + q0 + tid - t * G] * kLog2e;
-            }
-            named_bar_sync(1, kMassSum * 32);            // the log-sum-exps are everybody's
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_full);
-        };
-        if (chunks == 1) stage(0);
-        for (int t = first; t < last; ++t) {
-            const int j = t * kMassKeys + tid;
-            float sum = 0.f;
-            // the key's old weight, under way while the scores are formed
-            size_t cell = 0;
-            float old = 0.f;
-            bool real = j < keys;
-            if (real) {
-                const int page = pt[j / kPage];
-                real = page >= 0 && page < a.num_pages;
-                cell = plane + ((size_t)(real ? page : 0) * a.HK + kvh) * kPage + j % kPage;
-                if (real && j < L) old = a.mass[cell];
-            }
-            const int from = max(0, j - L) * G;          // rows that come before the key itself
-            for (int c = 0; c < chunks; ++c) {
-                if (chunks > 1) {
-                    wait(q_empty, qr.phase);             // the products of the rows before have read them ...
-                    qr.next();
-                    named_bar_sync(1, kMassSum * 32);    // ... and so have the sums
-                    stage(c);
-                }
-                wait(s_full(sr.i), sr.phase);
-                tc_fence_after();
+        for (long long x = begin; x < end;) {
+            const Run w = run_at(x);
+            x += w.last - w.first;
+            const int rows = w.kept * G, chunks = (rows + kMassRows - 1) / kMassRows;
+            const size_t plane = (size_t)w.layer * a.num_pages * a.HK * kPage;
+            const int* pt = a.page_table + (size_t)w.seq * a.max_pages;
+            auto stage = [&](int c) {            // rows c * 128 ..: into shared memory, with their log-sum-exps
+                wait(q_empty, qr.phase);         // the products of the rows before have read them ...
+                qr.next();
+                named_bar_sync(1, kMassSum * 32);        // ... and so have the sums
                 const int q0 = c * kMassRows, count = min(kMassRows, rows - q0);
-                for (int x = 0; x < count; x += 16) {
-                    float s[16];
-                    tc_ld16(lanes + sr.i * kMassRows + x, s);
-                    tc_wait_ld();
+                const size_t row0 = (size_t)w.layer * a.R + w.r0;
+                constexpr int B = 8, STEP = kMassSum * 32;       // loads in flight a thread
+                for (int e0 = tid; e0 < count * CPR; e0 += B * STEP) {
+                    uint4 v[B];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float p = fast_exp2(fmaf(s[e], a.scale_log2, -lse_s[x + e]));
-                        sum += x + e < count && q0 + x + e >= from ? p : 0.f;
+                    for (int k = 0; k < B; ++k) {
+                        const int e = min(e0 + k * STEP, count * CPR - 1), r = e / CPR, y = e % CPR, t = (q0 + r) / G;
+                        v[k] = *reinterpret_cast<const uint4*>(a.q + ((row0 + t) * a.H + w.kvh * G + q0 + r - t * G) * D + y * 8);
+                    }
+#pragma unroll
+                    for (int k = 0; k < B; ++k) {
+                        const int e = e0 + k * STEP, r = e / CPR, y = e % CPR;
+                        if (e < count * CPR) *reinterpret_cast<uint4*>(q_s + (y >> 3) * C::Q_SLAB + r * 128 + (((y ^ r) & 7) << 4)) = v[k];
                     }
                 }
-                tc_fence_before();
+                if (tid < count) {
+                    const int t = (q0 + tid) / G;
+                    lse_s[tid] = a.lse[(row0 + t) * a.H + w.kvh * G + q0 + tid - t * G] * kLog2e;
+                }
+                named_bar_sync(1, kMassSum * 32);            // the log-sum-exps are everybody's
+                fence_proxy_async();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(s_empty(sr.i));
-                sr.next();
-            }
-            if (real) {
-                a.mass[cell] = old + sum;
-                if (j >= L) a.pos[cell] = a.row_pos[r0 + j - L];
+                if (lane == 0) mbar_arrive(q_full);
+            };
+            if (chunks == 1) stage(0);
+            for (int t = w.first; t < w.last; ++t) {
+                const int j = t * kMassKeys + tid;
+                float sum = 0.f;
+                // the key's old weight, under way while the scores are formed
+                size_t cell = 0;
+                float old = 0.f;
+                bool real = j < w.keys;
+                if (real) {
+                    const int page = pt[j / kPage];
+                    real = page >= 0 && page < a.num_pages;
+                    cell = plane + ((size_t)(real ? page : 0) * a.HK + w.kvh) * kPage + j % kPage;
+                    if (real && j < w.L) old = a.mass[cell];
+                }
+                const int from = max(0, j - w.L) * G;        // rows that come before the key itself
+                for (int c = 0; c < chunks; ++c) {
+                    if (chunks > 1) stage(c);
+                    wait(s_full(sr.i), sr.phase);
+                    tc_fence_after();
+                    const int q0 = c * kMassRows, count = min(kMassRows, rows - q0);
+                    for (int y = 0; y < count; y += 16) {
+                        float s[16];
+                        tc_ld16(lanes + sr.i * kMassRows + y, s);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float p = fast_exp2(fmaf(s[e], a.scale_log2, -lse_s[y + e]));
+                            sum += y + e < count && q0 + y + e >= from ? p : 0.f;
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s_empty(sr.i));
+                    sr.next();
+                }
+                if (real) {
+                    a.mass[cell] = old + sum;
+                    if (j >= w.L) a.pos[cell] = a.row_pos[w.r0 + j - w.L];
+                }
             }
         }
     }
@@ -520,12 +570,9 @@ int launch_mass(const MassArgs& a, int layers, cudaStream_t st) {
     }
     CUtensorMap map;
     if (!describe_rows(&map, a.k_pages, D, (unsigned long long)layers * a.num_pages * a.HK * kPage, (size_t)D * 2, 1, (size_t)D * 2, false, kPage, 1, 1)) return TF_ECUDA;
-    // Blocks a column (layer, sequence, KV head): one round of the SMs where that many columns fit it (64 columns of 4096 keys, 2 blocks: 30 us, 3:
-    // 39, 10: 37), a few otherwise, so that columns of unequal length even out (256 columns of 2048 to 8192 keys: 172 us with 1, 152 with 2, 149 with 3).
-    const long long columns = (long long)layers * a.S * a.HK, tiles = (a.max_context + kMassKeys - 1) / kMassKeys;
-    const long long wanted = columns <= kSms ? kSms / columns : (3ll * kSms + columns - 1) / columns, blocks = wanted < tiles ? wanted : tiles;
+    const long long tiles = (long long)layers * a.S * a.HK * ((a.max_context + kMassKeys - 1) / kMassKeys);
     void* args[] = {const_cast<MassArgs*>(&a), &map};
-    if (launch_pdl((const void*)mass_kernel<D>, dim3((unsigned)blocks, a.HK, layers * a.S), dim3(kMassThreads), C::SMEM, st, args) != cudaSuccess) {
+    if (launch_pdl((const void*)mass_kernel<D>, dim3(tiles < kSms ? (unsigned)tiles : kSms), dim3(kMassThreads), C::SMEM, st, args) != cudaSuccess) {
         cudaGetLastError();
         return TF_ECUDA;
     }
@@ -548,7 +595,7 @@ int tf_attention_mass(const void* q, const float* lse, const void* k_pages, int 
     if (((uintptr_t)q | (uintptr_t)k_pages) & 15 || ((uintptr_t)mass | (uintptr_t)pos | (uintptr_t)lse) & 3) return TF_EALIGN;
     if ((long long)layers * n_seqs > 65535 || kv_heads > 65535 || (long long)layers * num_pages * kv_heads * 16 > 0x7FFFFFFFll) return TF_EINVAL;
     tf::MassArgs a{static_cast<const __nv_bfloat16*>(q), lse, static_cast<const __nv_bfloat16*>(k_pages), page_table, seq_lens, seq_start, keep,
-                   row_pos, mass, pos, status, num_pages, max_pages, heads, kv_heads, rows, n_seqs, max_context, scale * tf::kLog2e};
+                   row_pos, mass, pos, status, num_pages, max_pages, heads, kv_heads, rows, n_seqs, layers, max_context, scale * tf::kLog2e};
     return head_dim == 256 ? tf::launch_mass<256>(a, layers, static_cast<cudaStream_t>(stream)) : tf::launch_mass<128>(a, layers, static_cast<cudaStream_t>(stream));
 }
 
