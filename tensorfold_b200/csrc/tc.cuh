@@ -90,7 +90,7 @@ struct Waits {
 // the high one is the same for all operands here: next 8 rows 1024 bytes on, 128-byte swizzle. K-major operands ignore the leading
 // offset (1); for an MN-major one (V as the B operand: its rows are the contraction's index) it is the distance to the next 64 values.
 constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
-__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t leading) { return (addr >> 4) | leading << 16; }
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t leading) { return (addr & 0x3FFFFu) >> 4 | leading << 16; }      // (in a cluster the address names the block above bit 24)
 // D[tmem] (+)= A[smem] * B[smem], issued where `leader`
 __device__ __forceinline__ void tc_mma_ss(bool leader, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
     asm volatile(

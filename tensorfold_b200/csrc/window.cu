@@ -23,10 +23,15 @@
 // NaN, rows that do not keep their bits. Every step of a row's arithmetic is fixed by its own position and keys and by the chunk
 // size, so a row alone, in a window and as a serial step has the same bits.
 
+#include <cooperative_groups.h>
+
+#include <utility>
+
 #include "tc.cuh"
 
 namespace tf {
 namespace {
+namespace cg = cooperative_groups;
 
 constexpr int kPage = 16, kTile = 64, kRows = 128;     // keys a page, keys a tile, query rows a block (the tensor core's M)
 constexpr int kSoftWarps = 4, kMmaWarp = 4, kQWarp = 5, kKWarp = 6, kVWarp = 8, kProducers = 2, kThreads = 10 * 32, kSms = 148;
@@ -136,7 +141,7 @@ __device__ __forceinline__ Work work_of(const WindowArgs& a, int item, Raw raw, 
     w.sinks = a.sinks;
     w.tiles = 0;
     const int rows = min(a.group_rows, w.n - w.t0);
-    w.nq = rows * G;
+    w.nq = 0;
     if (w.n < 1) return w;
     if (w.n > a.max_window || w.L < 0 || w.L > a.max_context - w.n || w.r0 < 0 || w.r0 > a.R - w.n) {     // not what the call was made for
         if (speaks) report(a.status, TF_EINVAL);
@@ -145,6 +150,7 @@ __device__ __forceinline__ Work work_of(const WindowArgs& a, int item, Raw raw, 
     if (rows < 1) return w;
     w.p_first = w.L + w.t0;
     w.p_last = w.p_first + rows - 1;
+    w.nq = rows * G;
     w.lo_first = max(0, w.p_first + 1 - a.window);
     w.lo_last = max(0, w.p_last + 1 - a.window);
     int chunk = w.slot;
@@ -255,13 +261,81 @@ struct Cfg {
     static_assert((kRows - QR) * 128 <= (KS + VS) * TILE_BYTES, "the operand's rows lie inside the block's memory");
 };
 
+// The chunks of a row at slot p, joined in order, eight columns a lane: `read` fetches a slot's maximum, sum and columns, B at a time. Chunks in
+// which the row sees nothing are passed over, so the join does not depend on which chunks the rows beside it needed.
+template <int B, class Read>
+__device__ __forceinline__ void join_chunks(const WindowArgs& a, int p, Read read, float (&acc)[8], float& m, float& l) {
+    const int lo = max(0, p + 1 - a.window);
+    // chunks with sinks below the window, then the window's
+    const int head_chunks = min(a.sinks, lo) > 0 ? a.by_chunk(min(a.sinks, lo) - 1) + 1 : 0;
+    const int far = max(head_chunks, a.by_chunk(lo)), count = head_chunks + a.by_chunk(p) + 1 - far;
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+    for (int i0 = 0; i0 < count; i0 += B) {
+        float cm[B], cl[B];
+        float4 po[B][2];
+#pragma unroll
+        for (int k = 0; k < B; ++k) {
+            cl[k] = 0.f;
+            if (i0 + k >= count) continue;
+            const int i = i0 + k, chunk = i < head_chunks ? i : far + i - head_chunks;
+            read(slot_of(chunk, a.first_slots, a.near_slots), cm[k], cl[k], po[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < B; ++k) {
+            if (cl[k] == 0.f) continue;                                // NaN goes on
+            const float mn = fmaxf(m, cm[k]), sa = fast_exp2(m - mn), sb = fast_exp2(cm[k] - mn);      // m = -inf: sa = 0
+            const float x[8] = {po[k][0].x, po[k][0].y, po[k][0].z, po[k][0].w, po[k][1].x, po[k][1].y, po[k][1].z, po[k][1].w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] = fmaf(x[e], sb, acc[e] * sa);
+            l = fmaf(cl[k], sb, l * sa);
+            m = mn;
+        }
+    }
+}
+
+// A joined row on its way out. Whole warps (the packed form's group sums), `there`: this lane has a row.
+template <int D>
+__device__ __forceinline__ void finish_row(const WindowArgs& a, int row, int head, int li, bool there, const float (&acc)[8], float m, float l) {
+    if (a.lse != nullptr && li == 0 && there) a.lse[(size_t)row * a.H + head] = (m + log2f(l)) * kLn2;
+    const float inv = 1.f / l;               // (one chunk: the same operations as where the chunk kernel writes the results)
+    float o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = round_bf16(acc[e] * inv);
+    if (a.qg != nullptr && there) {
+        float g[8];
+        unpack8(*reinterpret_cast<const uint4*>(a.qg + (size_t)row * a.qg_stride + (size_t)head * 2 * D + D + li * 8), g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = round_bf16(o[e] * sigmoidf_(g[e]));
+    }
+    const uint4 v = pack8(o);
+    if (a.out != nullptr && there) *reinterpret_cast<uint4*>(a.out + ((size_t)row * a.H + head) * D + li * 8) = v;
+    if (a.out_packed != nullptr) {
+        const int Mp = tf_padded_rows(a.R), c8 = head * (D / 8) + li;
+        const float sum = a.group == 64 ? group_sum8<64>(v) : group_sum8<32>(v);
+        if (there) {
+            if (a.group == 64) packed_store<64>(a.out_packed, Mp, row, c8, v, sum);
+            else packed_store<32>(a.out_packed, Mp, row, c8, v, sum);
+        }
+    }
+}
+// Padding rows of the packed buffer are zero.
+__device__ __forceinline__ void zero_packed(const WindowArgs& a, int row, int c8) {
+    const int Mp = tf_padded_rows(a.R);
+    if (a.group == 64) packed_store<64>(a.out_packed, Mp, row, c8, make_uint4(0, 0, 0, 0), 0.f);
+    else packed_store<32>(a.out_packed, Mp, row, c8, make_uint4(0, 0, 0, 0), 0.f);
+}
+
 __device__ __forceinline__ float max3(float x, float y, float z) {
     float v;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(x), "f"(y), "f"(z));
     return v;
 }
 
-template <int D, int QR>
+// CLUSTER: the blocks of a cluster hold all chunks of a (sequence, KV head), one each, and join them through each other's shared memory.
+template <int D, int QR, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, blocks_of(D)) window_chunk_kernel(const __grid_constant__ WindowArgs a, const __grid_constant__ CUtensorMap q_map,
                                                                    const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                                                                    const __grid_constant__ CUtensorMap kn_map, const __grid_constant__ CUtensorMap vn_map) {
@@ -269,6 +343,9 @@ __global__ void __launch_bounds__(kThreads, blocks_of(D)) window_chunk_kernel(co
     constexpr int KS = C::KS, VS = C::VS, CPR = D / 8;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint32_t tmem_s;
+    __shared__ float2 sums_s[CLUSTER ? QR : 1];    // CLUSTER: maximum and sum of the block's rows; their values lie where K and V were
+    constexpr int JOIN_ROW = D * 4 + 16;
+    static_assert(!CLUSTER || QR * JOIN_ROW <= (KS + VS) * C::TILE_BYTES, "the rows' values fit");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint8_t* q_s = smem + ((1024u - (smem_u32(smem) & 1023u)) & 1023u);
     uint8_t* k_s = q_s + C::Q_BYTES;
@@ -589,6 +666,24 @@ __global__ void __launch_bounds__(kThreads, blocks_of(D)) window_chunk_kernel(co
             }
             // ---- the chunk's partials, or the results where a row has one chunk: 32 columns at a time through shared memory, so that a
             // store covers whole sectors ----
+            if constexpr (CLUSTER) {
+                if (mine) sums_s[tid] = make_float2(m, l);
+                wait(o_done((it - 1) & 1), (uint32_t)(((it - 1) >> 1) & 1));
+                tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    float o[32];
+                    tc_ld32(row + C::O_COL + c, o);
+                    tc_wait_ld();
+                    // fours in two halves, the even ones first: a reader's lanes, eight columns each, lie beside one another
+                    float4* to = reinterpret_cast<float4*>(k_s + tid * JOIN_ROW) + c / 8;
+                    if (tid < QR) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) to[(e & 1) * (D / 8) + (e >> 1)] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                    }
+                }
+                continue;
+            }
             const int rows_here = min(32, w.nq - warp * 32);
             constexpr int LANES = C::STAGE / 4, ROWS = 32 / LANES;       // lanes a row of partials, rows a store
             const size_t first = (size_t)w.slot * a.R * a.H;
@@ -646,15 +741,44 @@ __global__ void __launch_bounds__(kThreads, blocks_of(D)) window_chunk_kernel(co
         }
     }
     tc_fence_before();
-    __syncthreads();
+    if constexpr (CLUSTER) {
+        cg::cluster_group cluster = cg::this_cluster();
+        __syncwarp();
+        cluster.sync();
+        const Work w = work_of(a, blockIdx.x, fetch(a, blockIdx.x), false);
+        constexpr int LANES = D / 8;
+        const int G = (int)a.by_G.d, rank = (int)cluster.block_rank(), step = (int)cluster.num_blocks() * kThreads;
+        for (int i0 = rank * kThreads + warp * 32; i0 < w.nq * LANES; i0 += step) {
+            const int r = (i0 + lane) / LANES, li = lane % LANES;
+            const bool there = r < w.nq;
+            const int at = there ? r : 0, dt = a.by_G(at);
+            float acc[8], m, l;
+            join_chunks<4>(a, w.p_first + dt, [&](int slot, float& cm, float& cl, float4 (&x)[2]) {
+                const float2 sums = *cluster.map_shared_rank(&sums_s[at], slot);
+                const float4* src = reinterpret_cast<const float4*>(cluster.map_shared_rank(k_s, slot) + at * JOIN_ROW) + li;
+                cm = sums.x;
+                cl = sums.y;
+                x[0] = src[0];
+                x[1] = src[LANES];
+            }, acc, m, l);
+            finish_row<D>(a, w.r0 + w.t0 + dt, w.kvh * G + at - dt * G, li, there, acc, m, l);
+        }
+        auto others = cluster.barrier_arrive();
+        if (a.out_packed != nullptr && w.seq == 0 && rank == 0) {
+            const int pads = tf_padded_rows(a.R) - a.R, columns = G * LANES;
+            for (int i = tid; i < pads * columns; i += kThreads) zero_packed(a, a.R + i / columns, w.kvh * columns + i % columns);
+        }
+        cluster.barrier_wait(std::move(others));         // nobody leaves while another block may read its rows
+    } else {
+        __syncthreads();
+    }
     if (warp == kMmaWarp) {
         tc_fence_after();
         tc_dealloc(tmem, C::COLS);
     }
 }
 
-// Joins the chunks of a row, in order: D / 8 lanes a (row, head), eight values a lane. Chunks in which the row sees nothing are
-// passed over, so the join does not depend on which chunks the rows beside it needed.
+// Joins the chunks of the rows: D / 8 lanes a (row, head), B chunks in flight.
 template <int D, int B>
 __global__ void __launch_bounds__(128) window_join_kernel(const WindowArgs a) {
     constexpr int LANES = D / 8, PER_WARP = 32 / LANES;
@@ -662,85 +786,45 @@ __global__ void __launch_bounds__(128) window_join_kernel(const WindowArgs a) {
     pdl_wait();
     const int row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int head = (blockIdx.x * 4 + warp) * PER_WARP + lane / LANES, li = lane % LANES;
-    const int Mp = tf_padded_rows(a.R);
     int start = 0;
     const int seq = row < a.R ? seq_of(a.seq_start, a.S, row, start) : -1;
     const bool there = head < a.H;
-    const int c8 = head * LANES + li;
     if (seq < 0) {
-        if (row >= a.R && a.out_packed != nullptr && there) {          // padding rows of the packed buffer are zero
-            if (a.group == 64) packed_store<64>(a.out_packed, Mp, row, c8, make_uint4(0, 0, 0, 0), 0.f);
-            else packed_store<32>(a.out_packed, Mp, row, c8, make_uint4(0, 0, 0, 0), 0.f);
-        }
+        if (row >= a.R && a.out_packed != nullptr && there) zero_packed(a, row, head * LANES + li);
         return;
     }
     const int p = a.seq_lens[seq] + row - start;
     if (p < 0 || p >= a.max_context) return;                           // reported by the chunk kernel
-    const int lo = max(0, p + 1 - a.window);
-    // chunks with sinks below the window, then the window's
-    const int head_chunks = min(a.sinks, lo) > 0 ? a.by_chunk(min(a.sinks, lo) - 1) + 1 : 0;
-    const int far = max(head_chunks, a.by_chunk(lo)), count = head_chunks + a.by_chunk(p) + 1 - far;
-    float acc[8], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-    // B: chunks whose loads are in flight together
-    for (int i0 = 0; i0 < count; i0 += B) {
-        float cm[B], cl[B];
-        float4 po[B][2];
-#pragma unroll
-        for (int k = 0; k < B; ++k) {
-            cl[k] = 0.f;
-            if (i0 + k >= count) continue;
-            const int i = i0 + k, chunk = i < head_chunks ? i : far + i - head_chunks;
-            const size_t cell = ((size_t)slot_of(chunk, a.first_slots, a.near_slots) * a.R + row) * a.H + (there ? head : 0);
-            cm[k] = a.part_m[cell];
-            cl[k] = a.part_l[cell];
-            const float4* src = reinterpret_cast<const float4*>(a.part_o + cell * D + li * 8);
-            po[k][0] = src[0];
-            po[k][1] = src[1];
-        }
-#pragma unroll
-        for (int k = 0; k < B; ++k) {
-            if (cl[k] == 0.f) continue;                                // NaN goes on
-            const float mn = fmaxf(m, cm[k]), sa = fast_exp2(m - mn), sb = fast_exp2(cm[k] - mn);      // m = -inf: sa = 0
-            const float x[8] = {po[k][0].x, po[k][0].y, po[k][0].z, po[k][0].w, po[k][1].x, po[k][1].y, po[k][1].z, po[k][1].w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] = fmaf(x[e], sb, acc[e] * sa);
-            l = fmaf(cl[k], sb, l * sa);
-            m = mn;
-        }
-    }
-    if (a.lse != nullptr && li == 0 && there) a.lse[(size_t)row * a.H + head] = (m + log2f(l)) * kLn2;
-    const float inv = 1.f / l;               // (one chunk: the same operations as where the chunk kernel writes the results)
-    float o[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = round_bf16(acc[e] * inv);
-    if (a.qg != nullptr && there) {
-        float g[8];
-        unpack8(*reinterpret_cast<const uint4*>(a.qg + (size_t)row * a.qg_stride + (size_t)head * 2 * D + D + li * 8), g);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = round_bf16(o[e] * sigmoidf_(g[e]));
-    }
-    const uint4 v = pack8(o);
-    if (a.out != nullptr && there) *reinterpret_cast<uint4*>(a.out + ((size_t)row * a.H + head) * D + li * 8) = v;
-    if (a.out_packed != nullptr) {
-        const float sum = a.group == 64 ? group_sum8<64>(v) : group_sum8<32>(v);
-        if (there) {
-            if (a.group == 64) packed_store<64>(a.out_packed, Mp, row, c8, v, sum);
-            else packed_store<32>(a.out_packed, Mp, row, c8, v, sum);
-        }
-    }
+    float acc[8], m, l;
+    join_chunks<B>(a, p, [&](int slot, float& cm, float& cl, float4 (&x)[2]) {
+        const size_t cell = ((size_t)slot * a.R + row) * a.H + (there ? head : 0);
+        cm = a.part_m[cell];
+        cl = a.part_l[cell];
+        const float4* src = reinterpret_cast<const float4*>(a.part_o + cell * D + li * 8);
+        x[0] = src[0];
+        x[1] = src[1];
+    }, acc, m, l);
+    finish_row<D>(a, row, head, li, there, acc, m, l);
 }
 
 // ---- host side -----------------------------------------------------------------------------------------
-template <int D, int QR>
+// A cluster of a column's chunks joins them itself where rows and chunks are few and the clusters fit the GPU at once (of 148 SMs at least 7 of
+// 16 and 15 of 8). One row of 6 heads a KV head, 15 chunks of a window of 4096 keys: 13.9 us, with partials in memory and a second launch 15.0;
+// 4 chunks of 500 keys: 8.7 and 9.9. 24 query rows: 11.8 and 11.7; 48: 15.5 and 15.2, 11.0 and 10.1.
+bool clustered(const WindowArgs& a) {
+    const int columns = a.HK * a.S;
+    return a.qgroups == 1 && a.group_rows * (a.H / a.HK) <= 24 && a.slots >= 2 && a.slots <= 16 && columns <= (a.slots > 8 ? 7 : 15);
+}
+
+template <int D, int QR, bool CLUSTER>
 int launch_chunks(const WindowArgs& a, cudaStream_t st) {
     using C = Cfg<D, QR>;
     static bool configured[64] = {};       // the opt-in is per device
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return TF_ECUDA; }
     if (!configured[dev]) {
-        if (cudaFuncSetAttribute(window_chunk_kernel<D, QR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) {
+        if (cudaFuncSetAttribute(window_chunk_kernel<D, QR, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess ||
+            (CLUSTER && cudaFuncSetAttribute(window_chunk_kernel<D, QR, CLUSTER>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)) {
             cudaGetLastError();
             return TF_ECUDA;
         }
@@ -756,7 +840,8 @@ int launch_chunks(const WindowArgs& a, cudaStream_t st) {
         !describe_rows(&maps[4], a.v_new, D, R < 16 ? 16 : R, row * HK, HK, row, false, kPage, 1, D / 64))
         return TF_ECUDA;
     void* args[] = {const_cast<WindowArgs*>(&a), &maps[0], &maps[1], &maps[2], &maps[3], &maps[4]};
-    if (launch_pdl((const void*)window_chunk_kernel<D, QR>, dim3(a.items < a.blocks ? a.items : a.blocks), dim3(kThreads), C::SMEM, st, args) != cudaSuccess) {
+    if (launch_pdl((const void*)window_chunk_kernel<D, QR, CLUSTER>, dim3(a.items < a.blocks ? a.items : a.blocks), dim3(kThreads), C::SMEM, st, args, 0,
+                   CLUSTER ? a.slots : 1) != cudaSuccess) {
         cudaGetLastError();
         return TF_ECUDA;
     }
@@ -788,7 +873,8 @@ int run(WindowArgs& a, cudaStream_t st) {
         void* args[] = {&a};
         if (launch_pdl((const void*)window_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, args) != cudaSuccess) { cudaGetLastError(); return TF_ECUDA; }
     }
-    const int rc = a.group_rows * G <= 64 ? launch_chunks<D, 64>(a, st) : launch_chunks<D, 128>(a, st);
+    if (clustered(a)) return launch_chunks<D, 64, true>(a, st);
+    const int rc = a.group_rows * G <= 64 ? launch_chunks<D, 64, false>(a, st) : launch_chunks<D, 128, false>(a, st);
     if (rc != TF_OK || a.direct) return rc;
     void* join[] = {&a};
     const int heads = 4 * (32 / (D / 8)), out_rows = a.out_packed ? tf_padded_rows(a.R) : a.R;
@@ -855,7 +941,7 @@ int tf_window_launches(int rows, int n_seqs, int max_window, int slots, int head
     tf::WindowArgs a{};
     a.R = rows; a.S = n_seqs; a.max_window = max_window; a.slots = slots; a.H = heads; a.HK = kv_heads;
     a.blocks = tf::kSms * tf::blocks_of(head_dim);
-    return !tf::cut_rows(a) ? 0 : 1 + (tf::planned(a) ? 1 : 0) + (slots == 1 && plain ? 0 : 1);
+    return !tf::cut_rows(a) ? 0 : 1 + (tf::planned(a) ? 1 : 0) + ((slots == 1 && plain) || tf::clustered(a) ? 0 : 1);
 }
 
 int tf_window_attention(const void* q, const void* k_new, const void* v_new, const void* k_pages, const void* v_pages, int num_pages,

@@ -83,6 +83,7 @@ def test_launch_counts(lib):
     assert lib.tf_window_launches(128, 16, 8, 128, 24, 4, 256, 1) == 3             # 8192
     assert lib.tf_window_launches(128, 16, 8, 129, 24, 4, 256, 1) == 2
     assert lib.tf_window_launches(128, 16, 100, 20, 24, 4, 256, 1) == 3            # 5 groups of 21 rows
+    assert [lib.tf_window_launches(rows, 1, rows, slots, 24, 4, 256, 0) for rows, slots in ((1, 2), (4, 16), (5, 16), (1, 17))] == [1, 1, 2, 2]     # clusters
     assert [lib.tf_window_launches(1, seqs, 1, 1, 24, 4, 256, plain) for seqs, plain in ((2, 1), (2, 0), (60, 1), (60, 0))] == [1, 2, 2, 3]
     assert lib.tf_window_launches(0, 1, 1, 1, 1, 1, 128, 1) == lib.tf_window_launches(1, 1, 1, 1, 34, 2, 128, 1) == lib.tf_window_launches(1, 1 << 15, 1, 1 << 15, 4, 4, 128, 1) == 0
     assert lib.tf_window_launches(1, 1, 1, 74, 24, 4, 128, 1) == 2 and lib.tf_window_launches(1, 1, 1, 75, 24, 4, 128, 1) == 3      # two blocks an SM

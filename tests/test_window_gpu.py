@@ -275,3 +275,32 @@ def test_reports_and_refusals(lib):
     lane_window.window_attention(*args, **kw)
     with pytest.raises(RuntimeError):
         status.raise_if_set()
+
+
+@pytest.mark.parametrize("h,hk,d", [(24, 4, 256), (8, 2, 128), (6, 1, 256)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (300, 4)])
+def test_clusters_give_the_bits_of_the_join(lib, h, hk, d, window, sinks):
+    """One sequence alone, whose chunks a cluster joins, and among many, whose chunks go through memory; gate and packed rows, with the padding."""
+
+    from tensorfold_b200.lane_qmm import new_packed
+
+    lens, widths = [700, 515, 130, 3, 900, 64, 257, 800, 31, 555], [2, 1, 2, 1, 2, 1, 2, 1, 2, 1]
+    c = make(77, lens, widths, h, hk, d)
+    got, lse = attend(c, lens, widths, window, sinks, context=1000)
+    for s in range(len(lens)):
+        r0, w = int(c["start"][s]), widths[s]
+        one = dict(c, table=c["table"][s:s + 1].contiguous(), lens=c["lens"][s:s + 1].contiguous(), start=torch.tensor([0, w], dtype=torch.int32),
+                   **{n: c[n][r0:r0 + w].contiguous() for n in ("q", "k_new", "v_new")})
+        alone, lse1 = attend(one, lens[s:s + 1], [w], window, sinks, context=1000)
+        assert_same_bits(alone, got[r0:r0 + w])
+        assert_same_bits(lse1, lse[r0:r0 + w])
+        # packed rows, by a cluster and (beside nineteen sequences without rows) by the join
+        gate = torch.randn((w, h * 2 * d), generator=torch.Generator().manual_seed(s)).to(BF).cuda()
+        packs = []
+        for seqs in (1, 20):
+            many = dict(one, table=one["table"].repeat(seqs, 1), lens=one["lens"].repeat(seqs), start=torch.tensor([0] + [w] * seqs, dtype=torch.int32))
+            packed = new_packed(w, h * d, 64, "cuda")
+            packed.data.fill_(7)
+            attend(many, lens[s:s + 1] * seqs, [w], window, sinks, context=1000, out=None, gate=gate, packed_out=packed)
+            packs.append(packed.data.clone())
+        assert_same_bits(packs[0], packs[1])
