@@ -447,16 +447,18 @@ __global__ void __launch_bounds__(kChoiceThreads, 1) verify_choice_kernel(const 
     cluster.barrier_wait(std::move(others));     // nobody leaves while another block may read its sums
 }
 
-// Blocks a sequence: as many as still let all sequences' clusters run at the same time, which the GPU is asked once (of 148 SMs, for
-// instance, 7 clusters of 16, 15 of 8, 22 of 6 fit: 16 sequences as clusters of 8 took two rounds, 53 us against 50 of 6 at the time). Four where even those do not.
+// Blocks a sequence: as many as still let all sequences' clusters run at the same time, which the GPU is asked once. Of 148 SMs 7 clusters of 16,
+// 11 of 10, 15 of 9 (and of 8 or 7), 22 of 6, 26 of 5, 33 of 4 fit: 16 sequences as clusters of 8 took two rounds, 53 us against 50 of 6 at the
+// time; 24 of 5 take 78.6 us, of 4 84.8. All 26 of 5 do not always run at once (46 us without a drafter, 40 of 4): one less. Four where even those
+// do not fit.
 int cluster_for(int n_seqs) {
-    constexpr int kSizes[] = {16, 8, 6, kLeastBlocks};
-    static int fits[64][4];                      // per device; 0: not asked yet
+    constexpr int kSizes[] = {16, 10, 9, 6, 5, kLeastBlocks}, kCount = 6;
+    static int fits[64][kCount];                 // per device; 0: not asked yet
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return 0; }
-    if (fits[dev][3] == 0) {
+    if (fits[dev][kCount - 1] == 0) {
         if (cudaFuncSetAttribute(verify_choice_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) { cudaGetLastError(); return 0; }
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kCount; ++i) {
             cudaLaunchConfig_t cfg = {};
             cfg.gridDim = dim3(kSizes[i]);
             cfg.blockDim = dim3(kChoiceThreads);
@@ -471,9 +473,9 @@ int cluster_for(int n_seqs) {
             fits[dev][i] = n < 1 ? -1 : n;
         }
     }
-    for (int i = 0; i < 3; ++i)
-        if (fits[dev][i] >= n_seqs) return kSizes[i];
-    return fits[dev][3] > 0 ? kLeastBlocks : 0;
+    for (int i = 0; i + 1 < kCount; ++i)
+        if (fits[dev][i] - (kSizes[i] == 5) >= n_seqs) return kSizes[i];
+    return fits[dev][kCount - 1] > 0 ? kLeastBlocks : 0;
 }
 
 }  // namespace
