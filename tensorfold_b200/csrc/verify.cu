@@ -13,7 +13,7 @@
 // bound by the bytes of the logits (128 + 112 rows of 248320: 24 us, 5 TB/s). Choice: a cluster of blocks per sequence; every
 // block forms the acceptances from the slices' sums (64 bits), then the cluster goes over the one row that is drawn from, twice where a
 // drafter's distribution has to be normalised too - bound by the instructions of its 64-bit weights (16 rows of 248320 with a drafter:
-// 42 us; one row without, 11 us, mostly its dependent steps). An acceptance is one comparison, so 32-bit exponentials (relative
+// 39 us; one row without, 11 us, mostly its dependent steps). An acceptance is one comparison, so 32-bit exponentials (relative
 // error of p and q near 1e-6) decide all but one in a million draws as exact arithmetic would; a draw compares one number with
 // up to a million borders, so its weights and sums are in 64 bits throughout (relative error 1e-13). A NaN logit counts as -inf, +inf as a very
 // large one (tame).

@@ -5,17 +5,17 @@
 // log-sum-exp of the scores.
 //
 // The key axis is cut by ABSOLUTE position into chunks; a block handles one chunk of one (sequence, KV head) for up to 128 query
-// rows (window rows x the KV head's query heads, row = t * G + head), and a second kernel joins a row's chunks in order. In a block the
-// keys go by in tiles of 64:
+// rows (window rows x the KV head's query heads, row = t * G + head). A row's chunks are joined in order by a second kernel or, where rows and chunks are
+// few, by the cluster of blocks that holds them; a row of one chunk is finished by its block. In a block the keys go by in tiles of 64:
 //
 //   S = Q K^T        tcgen05, both operands in shared memory, 128 x 64 sums in tensor memory (two buffers)
-//   P = 2^(S - m)    four warps, a thread a row: no shuffles. m is a maximum that is only moved when a score exceeds it by 2^8, so the
+//   P = 2^(S - m)    four warps, a thread a row: no shuffles; P goes where S was, as bf16. m is a maximum that is only moved when a score exceeds it by 2^8, so the
 //                    sums so far are rescaled seldom (exactly the rows that need it change: multiplying by 1 keeps bits)
-//   O += P V         tcgen05, P in tensor memory as bf16, V in shared memory as it lies in the cache (rows are the contraction's index)
+//   O += P V         tcgen05, P in tensor memory, V in shared memory as it lies in the cache (rows are the contraction's index)
 //
 // What bounds it. Many users: memory (16 users, 2 to 8 rows, a window of 4096: 262 MB in 53 us, 4.9 TB/s, with 4 us before for the plan and 5
 // behind for the join). A prompt's rows with heads of 128: the chain scores - maximum - weights - product of a tile, of which two blocks an SM hide
-// a part (2900 rows, a window of 1024: 45 us for 19 GFLOP, 63 with one block and a join). One row: latency (11 us for 4096 keys).
+// a part (2900 rows, a window of 1024: 45 us for 19 GFLOP, 63 with one block and a join). One row: latency (10 us for a window of 1024 keys, 14 of 4096).
 //
 // K and V arrive by tiled copies (TMA), a page of 16 keys at a time, into rings of their own. A page that not all rows see whole
 // (around the committed length, the window's far edge, the sinks' end) is written by its producer warp instead, keys that no
