@@ -219,7 +219,8 @@ def sampled_decode(w: Weights, st: State, prompts: Sequence[Sequence[int]], pend
     max(p - q, 0) (``speculative.verify_drafts``): the tokens are distributed as serial sampling's, whatever the drafter proposes.
 
     ``draft(seq, context, k)`` returns up to k guesses, or (guesses, logits) with the (guesses, vocabulary) logits that they were drawn from
-    at ``draft_temperature`` (default: ``temperature``); guesses without logits, and the n-gram copies of the default drafter, are
+    at ``draft_temperature`` (default: ``temperature``), in bf16: a drafter with finer ones rounds them before it draws, since q has to be the
+    distribution of the draw. Guesses without logits, and the n-gram copies of the default drafter, are
     taken as certain (q = 1). ``generator``: of the uniform random numbers, on the weights' device.
     """
 
@@ -248,6 +249,8 @@ def sampled_decode(w: Weights, st: State, prompts: Sequence[Sequence[int]], pend
                 raise ValueError("sampled_decode: draft returned a token outside the vocabulary")
             if logits is not None and (logits.dim() != 2 or logits.shape[0] < len(guesses) or logits.shape[1] != w.config.vocab):
                 raise ValueError("sampled_decode: draft's logits must be (guesses, vocabulary)")
+            if logits is not None and logits.dtype != torch.bfloat16:
+                raise ValueError("sampled_decode: draft's logits must be bf16, and the guesses drawn from these values")
             if logits is not None and guesses:
                 given.append((len(rows) + 1, len(guesses), logits))
             rows += [out[s][-1]] + guesses

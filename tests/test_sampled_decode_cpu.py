@@ -1,0 +1,59 @@
+"""The round loop of ``decode.sampled_decode`` by itself, on the CPU: forward, verification and commit are stand-ins that note what they are given."""
+
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+VOCAB = 64
+
+
+@pytest.fixture
+def loop(monkeypatch):
+    """``loop.run(draft, count, seqs, ...)`` -> tokens; ``loop.calls``: the verifications' arguments; ``loop.commits``: what was committed."""
+
+    from tensorfold_b200 import decode
+
+    me = SimpleNamespace(calls=[], commits=[], keep=None, next=None, width=VOCAB)
+
+    def tree_forward(w, tokens, widths, st):
+        starts = [0]
+        for x in widths:
+            starts.append(starts[-1] + x)
+        start = torch.tensor(starts, dtype=torch.int32)
+        return torch.zeros((len(tokens), me.width), dtype=torch.bfloat16), SimpleNamespace(batch=SimpleNamespace(seq_start=start))
+
+    def verify_drafts(logits, tokens, seq_start, uniforms, **kw):
+        me.calls.append(SimpleNamespace(logits=logits, tokens=tokens, uniforms=uniforms, **kw))
+        widths = (seq_start[1:] - seq_start[:-1]).tolist()
+        keep = me.keep(widths) if me.keep else widths
+        token = me.next(widths) if me.next else [7 if x else -1 for x in widths]
+        return torch.tensor(keep, dtype=torch.int32), torch.tensor(token, dtype=torch.int32)
+
+    monkeypatch.setattr(decode, "tree_forward", tree_forward)
+    monkeypatch.setattr(decode, "verify_drafts", verify_drafts)
+    monkeypatch.setattr(decode, "commit", lambda st, rec, keep: me.commits.append(list(keep)))
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: None)
+
+    def run(draft, count=6, seqs=1, **kw):
+        w = SimpleNamespace(norm=torch.zeros(1), config=SimpleNamespace(vocab=VOCAB))
+        return decode.sampled_decode(w, SimpleNamespace(n_seqs=seqs), [[1, 2, 3]] * seqs, [4] * seqs, count, draft=draft, **kw).tokens
+
+    me.run = run
+    return me
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.float64, torch.int32])
+def test_drafters_logits_that_verification_would_round_are_refused(loop, dtype):
+    """q is the softmax of the logits that the guesses were drawn from; rounded to bf16 they are another distribution's."""
+
+    with pytest.raises(ValueError, match="bf16"):
+        loop.run(lambda s, ctx, k: ([5] * k, torch.zeros((k, VOCAB), dtype=dtype)))
+    assert not loop.commits
+
+
+def test_drafters_logits_reach_verification_as_they_are(loop):
+    theirs = torch.randn((8, VOCAB), generator=torch.Generator().manual_seed(0)).to(torch.bfloat16)
+    assert loop.run(lambda s, ctx, k: ([5] * k, theirs[:k]), seqs=2)[1] == [4] + [5] * 4 + [7]
+    near = loop.calls[0].draft_logits
+    assert near.dtype == torch.bfloat16 and torch.equal(near[1:5], theirs[:4]) and torch.equal(near[6:10], theirs[:4])
