@@ -57,3 +57,14 @@ def test_drafters_logits_reach_verification_as_they_are(loop):
     assert loop.run(lambda s, ctx, k: ([5] * k, theirs[:k]), seqs=2)[1] == [4] + [5] * 4 + [7]
     near = loop.calls[0].draft_logits
     assert near.dtype == torch.bfloat16 and torch.equal(near[1:5], theirs[:4]) and torch.equal(near[6:10], theirs[:4])
+
+
+def test_random_numbers_have_64_bits(loop):
+    """A vocabulary of 248320 has more borders than numbers of 24 bits tell apart evenly: 67 or 68 of them a token."""
+
+    loop.run(lambda s, ctx, k: [5] * k, count=80, seqs=2, generator=torch.Generator().manual_seed(3))
+    for call in loop.calls:
+        assert call.uniforms.dtype == torch.float64 and call.uniforms.shape == (len(call.tokens), 2)
+        assert bool(((call.uniforms >= 0) & (call.uniforms < 1)).all())
+    drawn = torch.cat([c.uniforms for c in loop.calls]).flatten() * 2.0 ** 24
+    assert float((drawn == drawn.floor()).double().mean()) < 0.01
