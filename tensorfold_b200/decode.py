@@ -221,7 +221,8 @@ def sampled_decode(w: Weights, st: State, prompts: Sequence[Sequence[int]], pend
     ``draft(seq, context, k)`` returns up to k guesses, or (guesses, logits) with the (guesses, vocabulary) logits that they were drawn from
     at ``draft_temperature`` (default: ``temperature``), in bf16: a drafter with finer ones rounds them before it draws, since q has to be the
     distribution of the draw. Guesses without logits, and the n-gram copies of the default drafter, are
-    taken as certain (q = 1). ``generator``: of the uniform random numbers, on the weights' device.
+    taken as certain (q = 1). ``generator``: of the uniform random numbers, on the weights' device. Logits that leave no token any probability
+    raise RuntimeError before that round is committed.
     """
 
     if count < 1 or not 1 <= max_rows <= MAX_ROWS:
@@ -268,6 +269,10 @@ def sampled_decode(w: Weights, st: State, prompts: Sequence[Sequence[int]], pend
         keep, token = verify_drafts(logits, tokens, rec.batch.seq_start, uniforms, temperature=temperature, draft_logits=near,
                                     draft_temperature=draft_temperature)
         keep, token = torch.stack([keep, token]).tolist()
+        none = [s for s in range(n) if widths[s] and token[s] < 0]
+        if none:
+            raise RuntimeError(f"sampled_decode: sequence {none[0]} at position {st.position(none[0]) + keep[none[0]]} has no token of any probability "
+                               "(logits all -inf or NaN)")
         r = 0
         for s in range(n):
             if widths[s]:

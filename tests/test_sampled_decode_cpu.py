@@ -37,7 +37,7 @@ def loop(monkeypatch):
 
     def run(draft, count=6, seqs=1, **kw):
         w = SimpleNamespace(norm=torch.zeros(1), config=SimpleNamespace(vocab=VOCAB))
-        return decode.sampled_decode(w, SimpleNamespace(n_seqs=seqs), [[1, 2, 3]] * seqs, [4] * seqs, count, draft=draft, **kw).tokens
+        return decode.sampled_decode(w, SimpleNamespace(n_seqs=seqs, position=lambda s: 3), [[1, 2, 3]] * seqs, [4] * seqs, count, draft=draft, **kw).tokens
 
     me.run = run
     return me
@@ -68,3 +68,22 @@ def test_random_numbers_have_64_bits(loop):
         assert bool(((call.uniforms >= 0) & (call.uniforms < 1)).all())
     drawn = torch.cat([c.uniforms for c in loop.calls]).flatten() * 2.0 ** 24
     assert float((drawn == drawn.floor()).double().mean()) < 0.01
+
+
+def test_a_row_without_probabilities_ends_the_run(loop):
+    """Verification answers -1 where every logit is -inf or NaN: no token, and nothing of that round is committed."""
+
+    rounds = iter([[9, 9], [9, -1], [9, 9]])
+    loop.next = lambda widths: next(rounds)
+    loop.keep = lambda widths: [1] * len(widths)
+    with pytest.raises(RuntimeError, match="sequence 1"):
+        loop.run(lambda s, ctx, k: [5] * k, seqs=2, count=20)
+    assert loop.commits == [[1, 1]]
+
+
+def test_sequences_that_are_done_have_no_token(loop):
+    """-1 is also what a sequence without rows gets."""
+
+    loop.keep = lambda widths: [x if s == 0 else min(x, 1) for s, x in enumerate(widths)]
+    tokens = loop.run(lambda s, ctx, k: [5] * k, seqs=2, count=6)
+    assert [len(t) for t in tokens] == [6, 6] and any(0 in c for c in loop.commits)
