@@ -244,7 +244,8 @@ def sampled_decode(w: Weights, st: State, prompts: Sequence[Sequence[int]], pend
                 continue
             k = max(min(max_rows, budget, count - len(out[s])) - 1, 0)
             made = draft(s, context[s], k) if draft is not None else copies[s].propose(context[s], k)
-            guesses, logits = made if isinstance(made, tuple) else (made, None)
+            pair = isinstance(made, tuple) and len(made) == 2 and (made[1] is None or torch.is_tensor(made[1]) and made[1].dim() > 0)
+            guesses, logits = made if pair else (made, None)
             guesses = [int(g) for g in guesses][:k]
             if any(not 0 <= g < w.config.vocab for g in guesses):
                 raise ValueError("sampled_decode: draft returned a token outside the vocabulary")

@@ -87,3 +87,12 @@ def test_sequences_that_are_done_have_no_token(loop):
     loop.keep = lambda widths: [x if s == 0 else min(x, 1) for s, x in enumerate(widths)]
     tokens = loop.run(lambda s, ctx, k: [5] * k, seqs=2, count=6)
     assert [len(t) for t in tokens] == [6, 6] and any(0 in c for c in loop.commits)
+
+
+def test_guesses_may_come_in_a_tuple(loop):
+    """A pair is guesses and logits only where its second part can be logits."""
+
+    for draft in (lambda s, ctx, k: (5, 6)[:k], lambda s, ctx, k: ((5, 6)[:k], None)):
+        loop.calls.clear()
+        assert loop.run(draft, count=4) == [[4, 5, 6, 7]]
+        assert loop.calls[0].draft_logits is None
