@@ -259,6 +259,7 @@ def sampled_decode(w: Weights, st: State, prompts: Sequence[Sequence[int]], pend
             widths.append(1 + len(guesses))
         tokens = _tokens(rows, dev)
         logits, rec = tree_forward(w, tokens, widths, st)
+        logits = logits[:, :w.config.vocab]    # the head's rows come in eights: what pads them is no token
         near = None
         if given:                              # guesses without logits beside some with: all of q on the guess
             near = torch.full_like(logits, float("-inf"))

@@ -96,3 +96,14 @@ def test_guesses_may_come_in_a_tuple(loop):
         loop.calls.clear()
         assert loop.run(draft, count=4) == [[4, 5, 6, 7]]
         assert loop.calls[0].draft_logits is None
+
+
+def test_padding_of_the_head_is_no_token(loop):
+    """A head's rows come in eights (a vocabulary of 61 has 64 logits): what lies behind the vocabulary takes no part."""
+
+    loop.width = VOCAB + 3
+    theirs = torch.zeros((8, VOCAB), dtype=torch.bfloat16)
+    assert len(loop.run(lambda s, ctx, k: ([5] * k, theirs[:k]))[0]) == 6
+    assert len(loop.run(lambda s, ctx, k: [5] * k)[0]) == 6
+    for call in loop.calls:
+        assert call.logits.shape[1] == VOCAB and (call.draft_logits is None or call.draft_logits.shape == call.logits.shape)
