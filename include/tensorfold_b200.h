@@ -320,7 +320,8 @@ int tf_lane_attention_paged_static(const void* q, const void* k_new, const void*
  * pages that no row sees are not read. max_window bounds a sequence's rows, max_context its keys with its window's own (also
  * reported). lse, when not NULL, receives ln(sum exp(score)) [rows, heads] fp32. Rows behind seq_start[n_seqs] are left as
  * they were in out and lse. out, qg, out_packed, group: as below for tf_lane_attention_paged_gated. Keys that no row may see (stale
- * rows of a page, later rows) may hold anything; a row that sees a value that is not finite has no specified result. */
+ * rows of a page, later rows) may hold anything; a row that sees a value that is not finite has no specified result in out, but
+ * its lse, which depends on keys alone. */
 int tf_window_chunk_keys(int n_seqs, int heads, int kv_heads, int max_window, int max_context, int window, int sinks);
 int tf_window_slots(int window, int sinks, int max_window, int max_context, int chunk_keys);
 size_t tf_window_scratch_bytes(int rows, int heads, int head_dim, int slots);

@@ -19,8 +19,8 @@
 //
 // K and V arrive by tiled copies (TMA), a page of 16 keys at a time, into rings of their own. A page that not all rows see whole
 // (around the committed length, the window's far edge, the sinks' end) is written by its producer warp instead, keys that no
-// row sees as zeros without being read. There a value that is not finite is written as zero and noted: rows that see its key become
-// NaN, rows that do not keep their bits. Every step of a row's arithmetic is fixed by its own position and keys and by the chunk
+// row sees as zeros without being read. There a value that is not finite is written as zero and noted: the results of rows that see its key become
+// NaN (their log-sum-exps, which do not depend on values, stay), rows that do not keep their bits. Every step of a row's arithmetic is fixed by its own position and keys and by the chunk
 // size, so a row alone, in a window and as a serial step has the same bits.
 
 #include <cooperative_groups.h>
@@ -580,6 +580,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(D)) window_chunk_kernel(co
                 // a part of the scores at a time, read twice where there are two (two blocks an SM have 96 registers a thread)
                 constexpr int PART = C::BLOCKS == 2 ? kTile / 2 : kTile;
                 uint32_t see[2] = {~0u, ~0u};            // bit e: the row sees key j0 + e; up to p, and from lo on or below the sinks' end
+                bool spoilt = false;                     // it sees a value that is not finite
                 if (!plain) {                            // the V tile's notes are there once it is (and stay until P V)
                     uint32_t bad[2] = {0, 0};
                     if (w.p_first != w.p_last) {         // (a row alone sees all that is read)
@@ -591,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(D)) window_chunk_kernel(co
                     const unsigned long long sees = below(p + 1 - j0) & (~below(lo - j0) | below(w.sinks - j0));
                     see[0] = (uint32_t)sees;
                     see[1] = (uint32_t)(sees >> 32);
-                    if ((see[0] & bad[0]) | (see[1] & bad[1])) l = __int_as_float(0x7FC00000);
+                    spoilt = ((see[0] & bad[0]) | (see[1] & bad[1])) != 0;
                 }
                 vr.next();
                 float s[PART];
@@ -653,6 +654,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(D)) window_chunk_kernel(co
                         const __nv_bfloat162 xy = __floats2bfloat162_rn(x, y);
                         pk[e >> 1] = *reinterpret_cast<const uint32_t*>(&xy);
                     }
+                    if (e0 == 0 && spoilt) pk[0] = 0x7FC07FC0u;     // NaN weights, of this row's results only
                     if constexpr (PART == kTile) tc_st32(row + C::S_COL + b * kTile, pk);
                     else tc_st16(row + C::S_COL + b * kTile + e0 / 2, pk);
                 }
