@@ -316,7 +316,7 @@ int tf_lane_attention_paged_static(const void* q, const void* k_new, const void*
  * on the GPU must not share it). tf_window_launches: how many kernels a call queues: the chunks, before them a plan where blocks take
  * several of them, behind them a join unless there is one slot and the call is plain (neither qg nor out_packed) or clusters of blocks join
  * (few rows, 2 to 16 slots). q, k_new, v_new, pages, out 16-byte aligned. num_pages bounds the page numbers: an entry
- * outside [0, num_pages) on a page that a row sees is reported as TF_EINVAL through `status` and its keys are left out; entries of
+ * outside [0, num_pages) on a page that a row sees is reported as TF_EINVAL through `status`, and the rows that see it become NaN; entries of
  * pages that no row sees are not read. max_window bounds a sequence's rows, max_context its keys with its window's own (also
  * reported). lse, when not NULL, receives ln(sum exp(score)) [rows, heads] fp32. Rows behind seq_start[n_seqs] are left as
  * they were in out and lse. out, qg, out_packed, group: as below for tf_lane_attention_paged_gated. Keys that no row may see (stale

@@ -19,9 +19,10 @@
 //
 // K and V arrive by tiled copies (TMA), a page of 16 keys at a time, into rings of their own. A page that not all rows see whole
 // (around the committed length, the window's far edge, the sinks' end) is written by its producer warp instead, keys that no
-// row sees as zeros without being read. There a value that is not finite is written as zero and noted: the results of rows that see its key become
-// NaN (their log-sum-exps, which do not depend on values, stay), rows that do not keep their bits. Every step of a row's arithmetic is fixed by its own position and keys and by the chunk
-// size, so a row alone, in a window and as a serial step has the same bits.
+// row sees as zeros without being read. There a value that is not finite is written as zero and noted: the results of rows that see its key
+// become NaN (their log-sum-exps, which do not depend on values, stay), rows that do not keep their bits. Keys on a page that is none
+// (reported) are NaN, and so are the rows that see them. Every step of a row's arithmetic is fixed by its own position and keys and by the
+// chunk size, so a row alone, in a window and as a serial step has the same bits.
 
 #include <cooperative_groups.h>
 
@@ -36,6 +37,7 @@ namespace cg = cooperative_groups;
 constexpr int kPage = 16, kTile = 64, kRows = 128;     // keys a page, keys a tile, query rows a block (the tensor core's M)
 constexpr int kSoftWarps = 4, kMmaWarp = 4, kQWarp = 5, kKWarp = 6, kVWarp = 8, kProducers = 2, kThreads = 10 * 32, kSms = 148;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr uint32_t kNan2 = 0x7FC07FC0u;                // two bf16 NaN
 constexpr float kSlack = 8.f;                          // how far (log2) a score may exceed the running maximum
 
 // n / d for 0 <= n < 2^31 without a division: d's reciprocal as a 32-bit fraction, rounded up (exact for n below 2^31 with the
@@ -474,6 +476,14 @@ __global__ void __launch_bounds__(kThreads, blocks_of(D)) window_chunk_kernel(co
                             }
                             if (__any_sync(0xffffffffu, odd)) bad |= 1u << at;
                         }
+                    } else {
+                        // a page that is none (reported): keys of NaN, and with them the scores of the rows that see it
+                        unsigned left = __ballot_sync(0xffffffffu, !(lane < kPage ? copy[0] : copy[1]) && w.any_sees(key) && lane < first_new && (lane < kPage ? num[0] : num[1]) < 0);
+                        for (; left != 0; left &= left - 1) {
+                            const int at = __ffs(left) - 1, r = at & (kPage - 1);
+                            if (lane / CPR == at % RPI)
+                                *reinterpret_cast<uint4*>(to + (at >> 4) * (kPage * 128) + r * 128 + (((c ^ r) & 7) << 4)) = make_uint4(kNan2, kNan2, kNan2, kNan2);
+                        }
                     }
                     if (is_v && lane == 0) bad_s[ring.i * 2 + half] = bad;
                     fence_proxy_async();
@@ -654,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(D)) window_chunk_kernel(co
                         const __nv_bfloat162 xy = __floats2bfloat162_rn(x, y);
                         pk[e >> 1] = *reinterpret_cast<const uint32_t*>(&xy);
                     }
-                    if (e0 == 0 && spoilt) pk[0] = 0x7FC07FC0u;     // NaN weights, of this row's results only
+                    if (e0 == 0 && spoilt) pk[0] = kNan2;     // NaN weights, of this row's results only
                     if constexpr (PART == kTile) tc_st32(row + C::S_COL + b * kTile, pk);
                     else tc_st16(row + C::S_COL + b * kTile + e0 / 2, pk);
                 }
