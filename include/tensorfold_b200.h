@@ -353,7 +353,9 @@ int tf_kv_commit(const void* k_new, const void* v_new, long long rec_stride, voi
  *   [layers, n_seqs, kv_heads] receives how many moved. seq_lens is not written: the caller's sequences now have
  *   min(length, budget) slots, whose order no longer follows the text.
  *   k_pages, v_pages, mass, pos 16-byte aligned. scratch: tf_evict_scratch_bytes, 4-byte aligned, no initialisation; two launches.
- * Calls that overlap on the GPU must not share a cache or scratch; a page belongs to one sequence. Both report a page number outside [0, num_pages) or a length above max_context as TF_EINVAL through `status` and leave those slots out. */
+ * Calls that overlap on the GPU must not share a cache or scratch; a page belongs to one sequence. Both report a page number outside [0, num_pages) as TF_EINVAL through `status`
+ * and leave its slots out. So does tf_attention_mass of a sequence of more than max_window rows or of more than max_context slots after the commit,
+ * which it leaves as it was, and tf_kv_evict of one of more than max_context slots, of which it leaves out what lies behind them. */
 int tf_attention_mass(const void* q, const float* lse, const void* k_pages, int num_pages, const int* page_table, int max_pages,
                       const int* seq_lens, const int* seq_start, const int* keep, const int* row_pos, float* mass, int* pos, int layers,
                       int rows, int n_seqs, int max_window, int max_context, int heads, int kv_heads, int head_dim, float scale, int* status,

@@ -25,7 +25,7 @@ struct MassArgs {
     float* mass;                   // [layers, pages, HK, 16]
     int* pos;
     int* status;
-    int num_pages, max_pages, H, HK, R, S, layers, max_context;
+    int num_pages, max_pages, H, HK, R, S, layers, max_window, max_context;
     float scale_log2;
 };
 
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kMassThreads, 1) mass_kernel(const __grid_cons
         if (s >= a.S) return make_int4(0, 0, 0, 0);
         const int r0 = a.seq_start[s], n = a.seq_start[s + 1] - r0, L = a.seq_lens[s], kept = min(max(a.keep[s], 0), n);
         if (kept < 1) return make_int4(0, 0, 0, 0);
-        if (r0 < 0 || r0 > a.R - n || L < 0 || L > a.max_context - kept || L > a.max_pages * kPage - kept) {
+        if (n > a.max_window || r0 < 0 || r0 > a.R - n || L < 0 || L > a.max_context - kept || L > a.max_pages * kPage - kept) {
             report(a.status, TF_EINVAL);
             return make_int4(0, 0, 0, 0);
         }
@@ -595,7 +595,7 @@ int tf_attention_mass(const void* q, const float* lse, const void* k_pages, int 
     if (((uintptr_t)q | (uintptr_t)k_pages) & 15 || ((uintptr_t)mass | (uintptr_t)pos | (uintptr_t)lse) & 3) return TF_EALIGN;
     if ((long long)layers * n_seqs > 65535 || kv_heads > 65535 || (long long)layers * num_pages * kv_heads * 16 > 0x7FFFFFFFll) return TF_EINVAL;
     tf::MassArgs a{static_cast<const __nv_bfloat16*>(q), lse, static_cast<const __nv_bfloat16*>(k_pages), page_table, seq_lens, seq_start, keep,
-                   row_pos, mass, pos, status, num_pages, max_pages, heads, kv_heads, rows, n_seqs, layers, max_context, scale * tf::kLog2e};
+                   row_pos, mass, pos, status, num_pages, max_pages, heads, kv_heads, rows, n_seqs, layers, max_window, max_context, scale * tf::kLog2e};
     return head_dim == 256 ? tf::launch_mass<256>(a, layers, static_cast<cudaStream_t>(stream)) : tf::launch_mass<128>(a, layers, static_cast<cudaStream_t>(stream));
 }
 

@@ -24,7 +24,8 @@ def attention_mass(q: torch.Tensor, lse: torch.Tensor, k_pages: torch.Tensor, pa
     k_pages (layers, pages, HK, 16, D); seq_lens (S,): the lengths before the commit; row_pos (R,): each row's position in the text;
     mass float32 and pos int32 (layers, pages, HK, 16), a cell per cached key. Every key gains the sum, over the kept rows that
     see it and its KV head's query heads, of exp(scale q . k - lse); the keys that the commit brought start at that sum and
-    take their row's position. ``max_window`` bounds a sequence's rows, ``max_context`` its slots after the commit.
+    take their row's position. ``max_window`` bounds a sequence's rows, ``max_context`` its slots after the commit; a sequence beyond
+    them is reported through the status word and left as it was.
     """
 
     _lib.need_cuda(q)
