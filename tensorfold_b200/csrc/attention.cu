@@ -450,7 +450,7 @@ int run(const AttnArgs& a, int n_seqs, int max_chunks, const int* row_nkeys, voi
     const bool two = D == 128 || columns < 16 || max_chunks * columns <= kSms;
     const void* kern = two ? (const void*)attn_chunk_kernel<D, 2> : (const void*)attn_chunk_kernel<D, D == 128 ? 2 : 1>;
     const auto bytes = [](int buffers) { return (kQRows + 2 * buffers * kTileKeys) * D * 2; };
-    static bool configured[64] = {};       // the opt-in is per device
+    static std::atomic<bool> configured[64] = {};       // the opt-in is per device
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return TF_ECUDA; }
     if (!configured[dev]) {

@@ -558,7 +558,7 @@ constexpr int kSms = 148;
 template <int D>
 int launch_mass(const MassArgs& a, int layers, cudaStream_t st) {
     using C = MassCfg<D>;
-    static bool configured[64] = {};       // the opt-in is per device
+    static std::atomic<bool> configured[64] = {};       // the opt-in is per device
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return TF_ECUDA; }
     if (!configured[dev]) {
@@ -621,7 +621,7 @@ int tf_kv_evict(void* k_pages, void* v_pages, int num_pages, const int* page_tab
     void* args[] = {&a};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool staged = max_context <= tf::kSelKeys;
-    static bool configured[64] = {};       // the opt-in is per device
+    static std::atomic<bool> configured[64] = {};       // the opt-in is per device
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return TF_ECUDA; }
     if (!configured[dev]) {

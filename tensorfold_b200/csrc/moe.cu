@@ -429,7 +429,7 @@ int tf_moe_group(const int* pick, int rows, int slots, int experts_total, int ma
     if (world < 1 || rank < 0 || rank >= world || experts < 1 || experts > experts_total) return TF_EINVAL;
     if (world > 1 && (experts % world || !prob_sel || !sel_count)) return TF_EINVAL;
     const size_t smem = (size_t)32 * experts_total * sizeof(unsigned short);      // up to 65 KB: the opt-in is per device
-    static bool configured[64] = {};
+    static std::atomic<bool> configured[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return TF_ECUDA; }
     if (!configured[dev]) {

@@ -677,7 +677,7 @@ int launch(const Args& a, cudaStream_t stream) {
     static_assert(C::SMEM <= 227 * 1024, "stage ring does not fit shared memory");
     auto kern = qmm_kernel<C, MULTI>;
     // the opt-in is per device: keep one flag per device ordinal
-    static bool configured[64] = {};
+    static std::atomic<bool> configured[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return TF_ECUDA; }
     if (!configured[dev]) {

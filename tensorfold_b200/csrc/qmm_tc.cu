@@ -509,7 +509,7 @@ int launch(const Args& a, cudaStream_t stream) {
     static_assert(C::SMEM <= 227 * 1024, "the rings do not fit shared memory");
     auto kern = qmm_kernel<G, NB, KTS, XS>;
     // the opt-in is per device: keep one flag per device ordinal
-    static bool configured[64] = {};
+    static std::atomic<bool> configured[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return TF_ECUDA; }
     if (!configured[dev]) {

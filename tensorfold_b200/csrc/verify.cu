@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(kChoiceThreads, 1) verify_choice_kernel(const 
 // do not fit.
 int cluster_for(int n_seqs) {
     constexpr int kSizes[] = {16, 10, 9, 6, 5, kLeastBlocks}, kCount = 6;
-    static int fits[64][kCount];                 // per device; 0: not asked yet
+    static std::atomic<int> fits[64][kCount];    // per device; the last one 0: not asked yet (threads that ask at the same time find the same)
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return 0; }
     if (fits[dev][kCount - 1] == 0) {

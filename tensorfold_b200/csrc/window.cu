@@ -831,7 +831,7 @@ bool clustered(const WindowArgs& a) {
 template <int D, int QR, bool CLUSTER>
 int launch_chunks(const WindowArgs& a, cudaStream_t st) {
     using C = Cfg<D, QR>;
-    static bool configured[64] = {};       // the opt-in is per device
+    static std::atomic<bool> configured[64] = {};       // the opt-in is per device
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return TF_ECUDA; }
     if (!configured[dev]) {
