@@ -12,8 +12,9 @@
 // Two launches. Row statistics: a slice of 8192 logits a block, an offset o, the largest y = logit * log2e / T, and the sum of 2^(y - o) -
 // bound by the bytes of the logits (128 + 112 rows of 248320: 24 us, 5 TB/s). Choice: a cluster of blocks per sequence; every
 // block forms the acceptances from the slices' sums (64 bits), then the cluster goes over the one row that is drawn from, twice where a
-// drafter's distribution has to be normalised too - bound by the instructions of its 64-bit weights (16 rows of 248320 with a drafter:
-// 39 us; one row without, 11 us, mostly its dependent steps). An acceptance is one comparison, so 32-bit exponentials (relative
+// drafter's distribution has to be normalised too. 16 rows of 248320 with a drafter: 39 us, on the 96 SMs that 16 clusters of 6 take and
+// with their 64-bit pipe busy 38 % of the time: the acceptances in front, loads that each warp waits for, the search and the cluster's
+// barriers are the rest. One row without a drafter: 11 us, mostly its dependent steps. An acceptance is one comparison, so 32-bit exponentials (relative
 // error of p and q near 1e-6) decide all but one in a million draws as exact arithmetic would; a draw compares one number with
 // up to a million borders, so its weights and sums are in 64 bits throughout (relative error 1e-13). A NaN logit counts as -inf, +inf as a very
 // large one (tame).
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
 // A weight 2^(logit c - offset) in 64 bits, in the two factors of which the second is a table's: t = 16 (logit c - offset) = n + r, a table of
 // 2^(j/16) times a factor of the row's own (128 bytes: no two entries share a bank; the high words less j << 16, so that adding n << 16 sets the
 // exponent), and the series of 2^(r/16) to the fifth power (the next term is 1.5e-13 at |r| = 1/2). Ten operations of the 64-bit pipe
-// with the product and eight others: the kernel is bound by how many instructions a weight takes. Weights end at 2^-900, which stands for 0 (NaN and
+// with the product and eight others (a pass over a row is its weights' instructions and its loads). Weights end at 2^-900, which stands for 0 (NaN and
 // -inf too): sums and weights up to kZero are none.
 constexpr int kTable = 16;
 constexpr double kZero = 1e-240;

@@ -39,10 +39,13 @@ def window_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, 
     """Attend (R, H, D) queries to each row's sequence: row t of sequence s stands at slot p = seq_lens[s] + t and sees key
     j <= p where p - j < ``window`` or j < ``sinks`` (``window`` None: every j <= p).
 
+    Softmax weights are rounded to bf16 for their product with V, as in ``lane_attention``; scores, sums and log-sum-exps are float32.
+
     k_new, v_new (R, HK, D) window rows; k_pages, v_pages (pages, HK, 16, D); page_table (S, max_pages), seq_lens (S,),
     seq_start (S+1,) int32 on the device. Table entries of pages that no row sees are never followed, so such pages may have been
     given back (``PagedKV.release_before``). ``max_window`` bounds a sequence's rows, ``max_context`` its keys with the window's
-    own; a sequence beyond them is reported through the status word. Rows behind the last sequence (R may exceed
+    own; a sequence beyond them is reported through the status word, and so is a page number that is none on a page that a row sees, which
+    makes the row NaN. Rows behind the last sequence (R may exceed
     seq_start[S]) are left as they were in ``out`` and ``lse``.
     ``lse``: float32 (R, H), receives ln(sum exp(score)) of each row and head. ``gate``, ``packed_out``, ``scratch``: as for
     ``lane_attention``. ``chunk_keys``: a multiple of 64; a row's bits depend on it and on the row's own keys, not on the rows

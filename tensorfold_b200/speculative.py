@@ -25,8 +25,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, seq_start: torch.T
     token is the first in vocabulary order whose cumulative weight exceeds uniforms[t, 1] of the total, t the last kept row: of
     max(p - q, 0) if the draft behind it was refused, of p if the window was kept whole. Full distributions: no top-k or top-p.
     Temperatures in 1e-6..1e6 (greedy decoding: ``sample_rows`` and ``accept_path``).
-    A sequence without rows gives (0, -1); a row without any probability keeps no draft and gives -1. ``max_window`` only has to be at
-    least the longest window and may be left out. ``keep`` is what ``kv_commit`` and ``lane_evict.attention_mass`` take.
+    A sequence without rows gives (0, -1); a row without any probability keeps no draft and gives -1. ``max_window`` (the longest window) is not
+    needed and changes nothing. ``keep`` is what ``kv_commit`` and ``lane_evict.attention_mass`` take.
     """
 
     if max_window is not None and max_window < 1:
